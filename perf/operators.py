@@ -14,6 +14,7 @@ Queries are N(0, 1), cached K and V N(0, 1) (int8: uniform codes, scales 0.01 to
 """
 import math
 
+import numpy as np
 import torch
 
 own = False
@@ -221,8 +222,9 @@ def _shared_plain(s):
 
 
 def _sample_plain(s):
-    """In 64 bits: a draw falls between two sums. Equal logits are kept or dropped together."""
-    c = s.case
+    """In 64 bits, with the settings as the 32-bit numbers that the call takes: a
+    draw falls between two sums. Equal logits are kept or dropped together."""
+    c = {k: float(np.float32(v)) if k in ("temperature", "top_p", "min_p") else v for k, v in s.case.items()}
     x = s.logits.double() / c["temperature"]
     e = torch.exp(x - x.amax(-1, keepdim=True))
     keep = torch.ones_like(e, dtype=torch.bool)
