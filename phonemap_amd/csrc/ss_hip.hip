@@ -573,6 +573,50 @@ int32_t attention_rows(ss_hip_ctx_t* c, float* out, const float* q, const void* 
   return 0;
 }
 
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// The context's device for the length of a call, and the caller's after it.
+struct DeviceScope {
+  int before = -1;
+  hipError_t status;
+  explicit DeviceScope(int device) {
+    status = hipGetDevice(&before);
+    if (status == hipSuccess && before == device) before = -1;
+    else if (status == hipSuccess) status = hipSetDevice(device);
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
+// What the window and the shared-prefix attention have in common; used: the cache is read.
+int32_t span_setup(ss_hip_ctx_t* c, const char* what, ssk::SpanArgs& a, float* out, const float* q, const void* kc,
+                   const void* vc, const float* ksc, const float* vsc, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                   float softcap, int32_t kv_type, bool used = true) {
+  if (!out || !q || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || (kv_type != 0 && kv_type != 1) ||
+      (kv_type == 1 && used && (!ksc || !vsc)) || !(softcap >= 0.f) || isinf(softcap))
+    return fail(kErrParams, "%s: bad argument", what);
+  if (!ssk::attention_supported(head_dim, n_heads / n_kv_heads))
+    return fail(kErrParams, "%s: head_dim %d / group %d not supported", what, head_dim, n_heads / n_kv_heads);
+  if (!aligned(out, 16) || !aligned(q, 16) || !aligned(kc, 16) || !aligned(vc, 16) || !aligned(ksc, 4) || !aligned(vsc, 4))
+    return fail(kErrParams, "%s: a pointer is not aligned (16 bytes; scales 4)", what);
+  memset(&a, 0, sizeof(a));
+  a.q = q;
+  a.out = out;
+  a.kc = kc;
+  a.vc = vc;
+  a.ks = ksc;
+  a.vs = vsc;
+  a.n_kv_heads = n_kv_heads;
+  a.scale = 1.0f / sqrtf((float)head_dim);
+  a.softcap = softcap;
+  a.softcap_inv = softcap > 0.f ? 1.0f / softcap : 0.f;
+  a.n_cu = c->n_cu;
+  return 0;
+}
+
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 }  // namespace
@@ -687,6 +731,109 @@ int32_t ss_hip_sample_logits(ss_hip_ctx_t* c, const float* logits, int32_t n, fl
   HIP_TRY(hipStreamSynchronize(s));
   *out_host = (int32_t)(uint32_t)(c->smp_io[0] & 0xffffffffu);
   if (temperature > 0.0f) *rng_state = c->smp_io[1];
+  return 0;
+}
+
+// ---- serving: windows, shared prompts, rows of logits ----
+size_t ss_hip_attention_window_workspace(ss_hip_ctx_t* c, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                         int32_t n_tokens, int32_t window, int32_t n_sinks) {
+  (void)c, (void)n_heads, (void)n_kv_heads, (void)head_dim, (void)n_tokens, (void)window, (void)n_sinks;
+  return 0;
+}
+
+int32_t ss_hip_attention_window(ss_hip_ctx_t* c, float* out, const float* q, const void* kc, const void* vc,
+                                const float* ksc, const float* vsc, int32_t n_heads, int32_t n_kv_heads,
+                                int32_t head_dim, int32_t max_seq, int32_t pos0, int32_t n_tokens, int32_t window,
+                                int32_t n_sinks, float softcap, int32_t kv_type, void* ws, size_t ws_bytes,
+                                void* stream) {
+  if (!c || !kc || !vc || pos0 < 0 || n_tokens <= 0 || (int64_t)pos0 + n_tokens > max_seq || window <= 0 || n_sinks < 0)
+    return fail(kErrParams, "attention_window: bad argument (pos0 %d, %d tokens, max_seq %d, window %d, %d sinks)", pos0,
+                n_tokens, max_seq, window, n_sinks);
+  ssk::SpanArgs a;
+  if (int32_t rc = span_setup(c, "attention_window", a, out, q, kc, vc, ksc, vsc, n_heads, n_kv_heads, head_dim, softcap,
+                              kv_type))
+    return rc;
+  a.max_seq = max_seq;
+  a.n = n_tokens;
+  a.pos0 = pos0;
+  a.window = window;
+  a.sinks = n_sinks;
+  (void)ws, (void)ws_bytes;
+  DeviceScope on(c->device);
+  HIP_TRY(on.status);
+  HIP_TRY(ssk::launch_span(head_dim, n_heads / n_kv_heads, kv_type, a, pick(c, stream)));
+  return 0;
+}
+
+size_t ss_hip_attention_shared_workspace(ss_hip_ctx_t* c, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                         int32_t n_seqs, int32_t prefix_len, int32_t own_max) {
+  (void)c, (void)n_heads, (void)n_kv_heads, (void)head_dim, (void)n_seqs, (void)prefix_len, (void)own_max;
+  return 0;
+}
+
+int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, const void* k_prefix, const void* v_prefix,
+                                const float* ks_prefix, const float* vs_prefix, int32_t prefix_max, int32_t prefix_len,
+                                const void* k_own, const void* v_own, const float* ks_own, const float* vs_own,
+                                int32_t own_max, const int32_t* own_len, int32_t n_seqs, int32_t n_heads,
+                                int32_t n_kv_heads, int32_t head_dim, float softcap, int32_t kv_type, void* ws,
+                                size_t ws_bytes, void* stream) {
+  if (!c || !k_own || !v_own || !own_len || n_seqs <= 0 || own_max <= 0 || prefix_len < 0 || prefix_len > prefix_max ||
+      (prefix_len > 0 && (!k_prefix || !v_prefix)))
+    return fail(kErrParams, "attention_shared: bad argument (%d sequences, prefix %d of %d, own_max %d)", n_seqs, prefix_len,
+                prefix_max, own_max);
+  ssk::SpanArgs a;
+  if (int32_t rc = span_setup(c, "attention_shared", a, out, q, k_prefix, v_prefix, ks_prefix, vs_prefix, n_heads, n_kv_heads,
+                              head_dim, softcap, kv_type, prefix_len > 0))
+    return rc;
+  if (kv_type == SS_HIP_KV_INT8 && (!ks_own || !vs_own)) return fail(kErrParams, "attention_shared: no scales");
+  if (!aligned(k_own, 16) || !aligned(v_own, 16) || !aligned(ks_own, 4) || !aligned(vs_own, 4) || !aligned(own_len, 4))
+    return fail(kErrParams, "attention_shared: a pointer is not aligned");
+  a.max_seq = prefix_max;
+  a.prefix = prefix_len;
+  a.n = n_seqs;
+  a.ko = k_own;
+  a.vo = v_own;
+  a.kos = ks_own;
+  a.vos = vs_own;
+  a.own_max = own_max;
+  a.own_len = own_len;
+  (void)ws, (void)ws_bytes;
+  DeviceScope on(c->device);
+  HIP_TRY(on.status);
+  HIP_TRY(ssk::launch_span(head_dim, n_heads / n_kv_heads, kv_type, a, pick(c, stream)));
+  return 0;
+}
+
+size_t ss_hip_sample_rows_workspace(ss_hip_ctx_t* c, int32_t n_rows, int32_t n) {
+  (void)c, (void)n_rows, (void)n;
+  return 0;
+}
+
+int32_t ss_hip_sample_rows(ss_hip_ctx_t* c, int32_t* out, const float* logits, int32_t n, int32_t n_rows, int64_t ld,
+                           float temperature, int32_t top_k, float top_p, float min_p, const float* u, void* ws,
+                           size_t ws_bytes, void* stream) {
+  if (!c || !out || !logits || !u || n <= 0 || n > ssk::kSampleRowsMaxV || n_rows <= 0 || n_rows > 65535 || ld < n)
+    return fail(kErrParams, "sample_rows: bad argument (%d rows of %d logits, stride %lld)", n_rows, n, (long long)ld);
+  if (!isfinite(temperature) || top_p != top_p || !(min_p <= 1.0f))
+    return fail(kErrParams, "sample_rows: temperature %g, top_p %g, min_p %g", temperature, top_p, min_p);
+  if (!aligned(out, 4) || !aligned(logits, 4) || !aligned(u, 4))
+    return fail(kErrParams, "sample_rows: a pointer is not aligned");
+  ssk::SampleRowsArgs a;
+  memset(&a, 0, sizeof(a));
+  a.logits = logits;
+  a.u = u;
+  a.out = out;
+  a.ld = ld;
+  a.V = n;
+  a.rows = n_rows;
+  a.temperature = temperature > 0.f ? temperature : 0.0;
+  a.top_k = top_k > 0 && top_k < n ? top_k : 0;
+  a.top_p = top_p > 0.f && top_p < 1.f ? top_p : 1.0;
+  a.min_gap = a.temperature > 0.0 && min_p > 0.f ? a.temperature * log((double)min_p) : -INFINITY;
+  (void)ws, (void)ws_bytes;
+  DeviceScope on(c->device);
+  HIP_TRY(on.status);
+  HIP_TRY(ssk::launch_sample_rows(a, pick(c, stream)));
   return 0;
 }
 

@@ -193,6 +193,35 @@ void gemm_launch_counts(int64_t* out, int n);
 // The workgroup shape of a product (nmat 2: EPI_SWIGLU): row tiles per workgroup, 1, 2 or 4.
 int gemm_shape(int rows, int T, int nmat, int cols, int type, int n_cu);
 bool attention_supported(int head_dim, int group);
+
+// Attention of rows whose keys are spans of one or two caches (ss_span.hip).
+// Window: row t is the token at position pos0 + t of one sequence; of the cache
+// kc / vc it sees the positions j <= pos0 + t with j < sinks or
+// j > pos0 + t - window. Shared: row t is the newest token of sequence t; it
+// sees the first `prefix` positions of kc / vc and the first own_len[t]
+// (0 .. own_max) positions of its own cache ko / vo.
+struct SpanArgs {
+  const float* q;            // [n][n_heads][hd]
+  float* out;                // the same
+  const void* kc;            // [n_kv_heads][max_seq][hd] fp16 or int8
+  const void* vc;
+  const float* ks;           // int8: scales [max_seq]
+  const float* vs;
+  const void* ko;            // shared: [n][n_kv_heads][own_max][hd]; window: null
+  const void* vo;
+  const float* kos;          // int8: scales [n][own_max]
+  const float* vos;
+  const int* own_len;        // device, [n]
+  int max_seq, own_max;
+  int n, n_kv_heads;
+  int pos0, window, sinks;   // window
+  int prefix;                // shared
+  float scale;
+  float softcap, softcap_inv;  // > 0: scores = softcap * tanh(scores * softcap_inv)
+  float* part;               // workspace of span_workspace() bytes
+  int n_cu;
+};
+hipError_t launch_span(int head_dim, int group, int kv_type, const SpanArgs& a, hipStream_t s);
 // positions one attention workgroup covers in one round of loads
 int attn_round_positions(int head_dim, int group);
 // attention workgroups of this shape resident on one compute unit (0: unknown)
@@ -252,6 +281,22 @@ struct SampleArgs {
 };
 size_t sample_scratch_bytes(int V);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t s);
+// The next token of every row of logits (ss_sample_rows.hip): temperature > 0
+// (0: the first maximum), top_k, top_p and min_p, and a random number per row.
+struct SampleRowsArgs {
+  const float* logits;       // [rows][ld]
+  const float* u;            // [rows]
+  int* out;                  // [rows]
+  int64_t ld;
+  int V, rows;
+  double temperature;
+  int top_k;                 // 0: off
+  double top_p;              // >= 1: off
+  double min_gap;            // T * log(min_p): the least x - max that stays (-inf: off)
+  void* work;                // sample_rows_workspace() bytes
+};
+constexpr int kSampleRowsMaxV = (1 << 19) - 1;   // sums of weights up to 2^44 stay below 2^63
+hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s);
 hipError_t launch_set_state(int* dpos, int* tokens, int pos, int token, hipStream_t s);
 hipError_t launch_advance(int* dpos, hipStream_t s);
 

@@ -1,0 +1,56 @@
+"""The serving calls refuse what they cannot compute, before any work on a
+device: the checks read the context's fields alone, so a block of zeros stands
+in for one. Every call here is refused."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import phonemap_amd as pm
+
+CTX = (C.c_uint8 * 4096)()
+P = 1 << 20   # an aligned address; nothing is read there
+
+WINDOW = dict(ctx=C.addressof(CTX), out=P, q=P, k=P, v=P, ks=None, vs=None, heads=8, kv_heads=2, hd=64, max_seq=100, pos0=10,
+              tokens=2, window=5, sinks=1, cap=0.0, kv=0, ws=P, ws_bytes=1 << 30, stream=None)
+SHARED = dict(ctx=C.addressof(CTX), out=P, q=P, kp=P, vp=P, ksp=None, vsp=None, prefix_max=50, prefix=20, ko=P, vo=P, kso=None,
+              vso=None, own_max=10, lens=P, seqs=2, heads=8, kv_heads=2, hd=64, cap=0.0, kv=0, ws=P, ws_bytes=1 << 30, stream=None)
+SAMPLE = dict(ctx=C.addressof(CTX), out=P, logits=P, n=100, rows=2, ld=100, temperature=1.0, top_k=5, top_p=0.9, min_p=0.1, u=P,
+              ws=P, ws_bytes=1 << 30, stream=None)
+
+
+def _refused(name, good, **bad):
+    L = pm.lib()
+    assert getattr(L, name)(*{**good, **bad}.values()) == -5, bad
+    assert L.ss_hip_last_error().decode().startswith(name[len("ss_hip_"):] + ":"), L.ss_hip_last_error()
+
+
+@pytest.mark.parametrize("bad", [
+    dict(ctx=None), dict(out=None), dict(q=None), dict(k=None), dict(v=None), dict(heads=0), dict(heads=7), dict(heads=-8),
+    dict(kv_heads=0), dict(kv_heads=-2), dict(heads=6), dict(hd=96), dict(hd=0), dict(heads=32), dict(pos0=-1), dict(tokens=0),
+    dict(tokens=-1), dict(pos0=99), dict(pos0=2 ** 31 - 1), dict(tokens=2 ** 31 - 1), dict(window=0), dict(window=-1),
+    dict(sinks=-1), dict(cap=-1.0), dict(cap=float("nan")), dict(cap=float("inf")), dict(kv=2), dict(kv=-1), dict(kv=1),
+    dict(kv=1, ks=P), dict(kv=1, vs=P), dict(q=P + 4), dict(out=P + 8), dict(k=P + 2), dict(v=P + 1), dict(kv=1, ks=P + 2, vs=P),
+], ids=str)
+def test_window(bad):
+    _refused("ss_hip_attention_window", WINDOW, **bad)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(ctx=None), dict(out=None), dict(q=None), dict(kp=None), dict(vp=None), dict(ko=None), dict(vo=None), dict(lens=None),
+    dict(prefix=-1), dict(prefix=51), dict(own_max=0), dict(own_max=-1), dict(seqs=0), dict(seqs=-1), dict(heads=7), dict(hd=32),
+    dict(heads=32), dict(cap=float("nan")), dict(kv=3), dict(kv=1), dict(kv=1, ksp=P, vsp=P), dict(kv=1, kso=P, vso=P),
+    dict(kv=1, ksp=P, vsp=P, kso=P), dict(ko=P + 8), dict(vo=P + 2), dict(kp=P + 2), dict(lens=P + 2),
+    dict(kv=1, ksp=P, vsp=P, kso=P, vso=P + 1),
+], ids=str)
+def test_shared(bad):
+    _refused("ss_hip_attention_shared", SHARED, **bad)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(ctx=None), dict(out=None), dict(logits=None), dict(u=None), dict(n=0), dict(n=-1), dict(n=1 << 19, ld=1 << 19),
+    dict(rows=0), dict(rows=-1), dict(rows=65536), dict(ld=99), dict(temperature=float("nan")), dict(temperature=float("inf")),
+    dict(top_p=float("nan")), dict(min_p=float("nan")), dict(min_p=1.5), dict(logits=P + 2), dict(u=P + 1), dict(out=P + 2),
+], ids=str)
+def test_sample(bad):
+    _refused("ss_hip_sample_rows", SAMPLE, **bad)
