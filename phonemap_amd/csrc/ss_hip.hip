@@ -591,15 +591,30 @@ struct DeviceScope {
   DeviceScope& operator=(const DeviceScope&) = delete;
 };
 
+// rows that the serving attention takes: query rows and outputs that 32 bits count
+bool span_shape_ok(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t n) {
+  return n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n > 0 &&
+         ssk::attention_supported(head_dim, n_heads / n_kv_heads) && (int64_t)n * n_heads <= (1 << 24);
+}
+
+int32_t span_scratch(const char* what, ssk::SpanArgs& a, void* ws, size_t have, size_t need) {
+  if (need && (!ws || have < need || !aligned(ws, 16)))
+    return fail(kErrParams, "%s: needs a 16-byte aligned workspace of %zu bytes (%zu given)", what, need, ws ? have : (size_t)0);
+  a.part = static_cast<float*>(ws);
+  return 0;
+}
+
 // What the window and the shared-prefix attention have in common; used: the cache is read.
 int32_t span_setup(ss_hip_ctx_t* c, const char* what, ssk::SpanArgs& a, float* out, const float* q, const void* kc,
                    const void* vc, const float* ksc, const float* vsc, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
-                   float softcap, int32_t kv_type, bool used = true) {
+                   int32_t n, float softcap, int32_t kv_type, bool used = true) {
   if (!out || !q || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || (kv_type != 0 && kv_type != 1) ||
       (kv_type == 1 && used && (!ksc || !vsc)) || !(softcap >= 0.f) || isinf(softcap))
     return fail(kErrParams, "%s: bad argument", what);
   if (!ssk::attention_supported(head_dim, n_heads / n_kv_heads))
     return fail(kErrParams, "%s: head_dim %d / group %d not supported", what, head_dim, n_heads / n_kv_heads);
+  if (!span_shape_ok(n_heads, n_kv_heads, head_dim, n))
+    return fail(kErrParams, "%s: %d rows of %d heads are too many", what, n, n_heads);
   if (!aligned(out, 16) || !aligned(q, 16) || !aligned(kc, 16) || !aligned(vc, 16) || !aligned(ksc, 4) || !aligned(vsc, 4))
     return fail(kErrParams, "%s: a pointer is not aligned (16 bytes; scales 4)", what);
   memset(&a, 0, sizeof(a));
@@ -610,6 +625,7 @@ int32_t span_setup(ss_hip_ctx_t* c, const char* what, ssk::SpanArgs& a, float* o
   a.ks = ksc;
   a.vs = vsc;
   a.n_kv_heads = n_kv_heads;
+  while (n_kv_heads << a.gs < n_heads) ++a.gs;   // (groups of 1, 2, 4 or 8)
   a.scale = 1.0f / sqrtf((float)head_dim);
   a.softcap = softcap;
   a.softcap_inv = softcap > 0.f ? 1.0f / softcap : 0.f;
@@ -737,8 +753,8 @@ int32_t ss_hip_sample_logits(ss_hip_ctx_t* c, const float* logits, int32_t n, fl
 // ---- serving: windows, shared prompts, rows of logits ----
 size_t ss_hip_attention_window_workspace(ss_hip_ctx_t* c, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                          int32_t n_tokens, int32_t window, int32_t n_sinks) {
-  (void)c, (void)n_heads, (void)n_kv_heads, (void)head_dim, (void)n_tokens, (void)window, (void)n_sinks;
-  return 0;
+  if (!c || !span_shape_ok(n_heads, n_kv_heads, head_dim, n_tokens) || window <= 0 || n_sinks < 0) return 0;
+  return ssk::span_window_workspace(head_dim, n_heads / n_kv_heads, n_kv_heads, n_tokens, window, n_sinks, c->n_cu);
 }
 
 int32_t ss_hip_attention_window(ss_hip_ctx_t* c, float* out, const float* q, const void* kc, const void* vc,
@@ -750,25 +766,27 @@ int32_t ss_hip_attention_window(ss_hip_ctx_t* c, float* out, const float* q, con
     return fail(kErrParams, "attention_window: bad argument (pos0 %d, %d tokens, max_seq %d, window %d, %d sinks)", pos0,
                 n_tokens, max_seq, window, n_sinks);
   ssk::SpanArgs a;
-  if (int32_t rc = span_setup(c, "attention_window", a, out, q, kc, vc, ksc, vsc, n_heads, n_kv_heads, head_dim, softcap,
-                              kv_type))
+  if (int32_t rc = span_setup(c, "attention_window", a, out, q, kc, vc, ksc, vsc, n_heads, n_kv_heads, head_dim, n_tokens,
+                              softcap, kv_type))
     return rc;
   a.max_seq = max_seq;
   a.n = n_tokens;
   a.pos0 = pos0;
-  a.window = window;
-  a.sinks = n_sinks;
-  (void)ws, (void)ws_bytes;
+  a.window = window < max_seq ? window : max_seq;
+  a.sinks = n_sinks < max_seq ? n_sinks : max_seq;
+  if (int32_t rc = span_scratch("attention_window", a, ws, ws_bytes,
+                                ss_hip_attention_window_workspace(c, n_heads, n_kv_heads, head_dim, n_tokens, window, n_sinks)))
+    return rc;
   DeviceScope on(c->device);
   HIP_TRY(on.status);
-  HIP_TRY(ssk::launch_span(head_dim, n_heads / n_kv_heads, kv_type, a, pick(c, stream)));
+  HIP_TRY(ssk::launch_span(head_dim, kv_type, a, pick(c, stream)));
   return 0;
 }
 
 size_t ss_hip_attention_shared_workspace(ss_hip_ctx_t* c, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                          int32_t n_seqs, int32_t prefix_len, int32_t own_max) {
-  (void)c, (void)n_heads, (void)n_kv_heads, (void)head_dim, (void)n_seqs, (void)prefix_len, (void)own_max;
-  return 0;
+  if (!c || !span_shape_ok(n_heads, n_kv_heads, head_dim, n_seqs) || prefix_len < 0 || own_max <= 0) return 0;
+  return ssk::span_shared_workspace(head_dim, n_heads / n_kv_heads, n_kv_heads, n_seqs, prefix_len, own_max, c->n_cu);
 }
 
 int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, const void* k_prefix, const void* v_prefix,
@@ -783,7 +801,7 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, con
                 prefix_max, own_max);
   ssk::SpanArgs a;
   if (int32_t rc = span_setup(c, "attention_shared", a, out, q, k_prefix, v_prefix, ks_prefix, vs_prefix, n_heads, n_kv_heads,
-                              head_dim, softcap, kv_type, prefix_len > 0))
+                              head_dim, n_seqs, softcap, kv_type, prefix_len > 0))
     return rc;
   if (kv_type == SS_HIP_KV_INT8 && (!ks_own || !vs_own)) return fail(kErrParams, "attention_shared: no scales");
   if (!aligned(k_own, 16) || !aligned(v_own, 16) || !aligned(ks_own, 4) || !aligned(vs_own, 4) || !aligned(own_len, 4))
@@ -797,10 +815,12 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, con
   a.vos = vs_own;
   a.own_max = own_max;
   a.own_len = own_len;
-  (void)ws, (void)ws_bytes;
+  if (int32_t rc = span_scratch("attention_shared", a, ws, ws_bytes,
+                                ss_hip_attention_shared_workspace(c, n_heads, n_kv_heads, head_dim, n_seqs, prefix_len, own_max)))
+    return rc;
   DeviceScope on(c->device);
   HIP_TRY(on.status);
-  HIP_TRY(ssk::launch_span(head_dim, n_heads / n_kv_heads, kv_type, a, pick(c, stream)));
+  HIP_TRY(ssk::launch_span(head_dim, kv_type, a, pick(c, stream)));
   return 0;
 }
 

@@ -214,14 +214,18 @@ struct SpanArgs {
   const int* own_len;        // device, [n]
   int max_seq, own_max;
   int n, n_kv_heads;
+  int gs;                    // log2 of the query heads per KV head
   int pos0, window, sinks;   // window
   int prefix;                // shared
   float scale;
   float softcap, softcap_inv;  // > 0: scores = softcap * tanh(scores * softcap_inv)
-  float* part;               // workspace of span_workspace() bytes
+  float* part;               // workspace, as the functions below size it
   int n_cu;
 };
-hipError_t launch_span(int head_dim, int group, int kv_type, const SpanArgs& a, hipStream_t s);
+hipError_t launch_span(int head_dim, int kv_type, const SpanArgs& a, hipStream_t s);
+// bytes of SpanArgs::part; window and sinks at most max_seq
+size_t span_window_workspace(int head_dim, int group, int n_kv_heads, int n, int window, int sinks, int n_cu);
+size_t span_shared_workspace(int head_dim, int group, int n_kv_heads, int n, int prefix, int own_max, int n_cu);
 // positions one attention workgroup covers in one round of loads
 int attn_round_positions(int head_dim, int group);
 // attention workgroups of this shape resident on one compute unit (0: unknown)
