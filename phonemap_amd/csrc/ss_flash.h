@@ -78,6 +78,7 @@
 #include "ss_device.h"
 #include "ss_kernels.h"
 #include "ss_mfma.h"
+#include "ss_span.h"
 
 namespace ssk {
 
@@ -153,8 +154,18 @@ __device__ __forceinline__ void one_row(const AttnArgs& a, const float* q, const
   for (int d = 0; d < ND; ++d) out[lane + kWave * d] = o[d] / l;
 }
 
-template <int HD, int G, int RT, int KG, int DS, bool Q8, bool FULL>
-__global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs a) {
+// Rows that see a window and the first positions rather than all up to their own.
+// Their keys can be left to `slots` workgroups, whose shares k_span_join joins.
+struct SpanRows : AttnArgs {
+  SpanArgs s;
+  int slots;
+};
+__device__ __forceinline__ constexpr bool leaves_share(const AttnArgs&) { return false; }
+__device__ __forceinline__ bool leaves_share(const SpanRows& a) { return a.slots > 1; }
+
+template <int HD, int G, int RT, int KG, int DS, bool Q8, bool FULL, class Args = AttnArgs>
+__global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const Args a) {
+  constexpr bool SPAN = !std::is_same_v<Args, AttnArgs>;
   constexpr int CH = HD / 8;             // 16-byte chunks per row
   constexpr int NC = HD / 16 / DS;       // a wave's 16-wide slices of the head dimension
   constexpr int NDT = HD / 32 / DS;      // and 32-dim tiles of O^T
@@ -162,7 +173,7 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
   constexpr int kGrp = kBlk * CH;        // chunks of one key group's block
   constexpr int kLoads = kGrp / (64 * RT * DS);   // direct loads per wave, K and V each
   static_assert(HD == 64 || HD == 128 || HD == 256, "head_dim 64, 128 or 256");
-  static_assert(kBlk % G == 0 && RT <= 2 && KG % 2 == 0 && kGrp % (64 * RT * DS) == 0, "shape");
+  static_assert((SPAN || kBlk % (G ? G : 1) == 0) && RT <= 2 && KG % 2 == 0 && kGrp % (64 * RT * DS) == 0, "shape");
 
   // two buffers of each, as separate arrays: the loop names them at compile
   // time, so the compiler can tell the buffer being read from the one the
@@ -181,22 +192,72 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
   // neighbouring workgroups take the KV heads in turn, so the workgroups of
   // one head meet in one XCD's L2; the longest prefixes come first
   const int kvh = blockIdx.x % a.n_kv_heads;
-  const int row0 = (gridDim.x / a.n_kv_heads - 1 - blockIdx.x / a.n_kv_heads) * (RT * 32);
+  int row0, slot = 0;
+  if constexpr (SPAN) {
+    row0 = blockIdx.x / (a.n_kv_heads * a.slots) * (RT * 32);
+    slot = blockIdx.x / a.n_kv_heads % a.slots;
+  } else {
+    row0 = (gridDim.x / a.n_kv_heads - 1 - blockIdx.x / a.n_kv_heads) * (RT * 32);
+  }
+  // token and head of a query row of the KV head's group
+  auto token = [&](int r) {
+    if constexpr (SPAN) return r >> a.s.gs;
+    else return r / G;
+  };
+  auto head_of = [&](int r) {
+    if constexpr (SPAN) return r & ((1 << a.s.gs) - 1);
+    else return r % G;
+  };
+  auto head_at = [&](int hr) -> size_t {   // head hr of the KV head's among a token's values
+    if constexpr (SPAN) return (((size_t)kvh << a.s.gs) + hr) * HD;
+    else return ((size_t)kvh * G + hr) * HD;
+  };
 
   // this lane's query row: token z, head hq of the KV head's group
   const int row = row0 + 32 * rt + n;
-  const int z = row / G, hq = row % G;
-  const int lim = a.pos0 + z;   // last position the row sees (rows past the last token are not stored)
-  // positions 0..ctx-1 serve every token of the workgroup; wmin..wmax are this wave's rows' limits
-  const int ctx = a.pos0 + min((row0 + RT * 32 - 1) / G, a.n_tok - 1) + 1;
-  const int wmin = a.pos0 + (row0 + 32 * rt) / G, wmax = min(wmin + 32 / G, ctx) - 1;
-  const int nstep = (ctx + KG * kBlk - 1) / (KG * kBlk);
+  const int z = token(row), hq = head_of(row);
+  int lim, ctx, wmin, wmax, nstep;
+  Walk wk = {};   // SPAN: the blocks some row of the workgroup sees
+  int low = 0, wlow = 0;
+  if constexpr (!SPAN) {
+    lim = a.pos0 + z;   // last position the row sees (rows past the last token are not stored)
+    // positions 0..ctx-1 serve every token of the workgroup; wmin..wmax are this wave's rows' limits
+    ctx = a.pos0 + min(token(row0 + RT * 32 - 1), a.n_tok - 1) + 1;
+    wmin = a.pos0 + token(row0 + 32 * rt), wmax = min(wmin + 32 / G, ctx) - 1;
+    nstep = (ctx + KG * kBlk - 1) / (KG * kBlk);
+  } else {
+    const int last = a.n_tok - 1;
+    ctx = a.pos0 + min(token(row0 + RT * 32 - 1), last) + 1;
+    lim = a.pos0 + min(z, last);
+    wmin = a.pos0 + min(token(row0 + 32 * rt), last), wmax = a.pos0 + min(token(row0 + 32 * rt + 31), last);
+    low = lim - a.s.window;       // positions up to here: the first ones alone
+    wlow = wmax - a.s.window;     // the highest of this wave's
+    wk.to0 = min(a.s.sinks, ctx);
+    wk.from1 = max(wk.to0, a.pos0 + token(row0) + 1 - a.s.window);
+    wk.to1 = ctx;
+    wk.nb0 = (wk.to0 + kBlk - 1) / kBlk;
+    wk.nb = wk.nb0 + (wk.to1 - wk.from1 + kBlk - 1) / kBlk;
+    const int mine = (wk.nb + KG - 1) / KG;   // steps of all slots, taken in turn
+    nstep = (mine - slot + a.slots - 1) / a.slots;
+  }
+  // this group's block of a step: positions kb .. end - 1 (kBlk of them or fewer), false: none
+  auto block = [&](int step, int& kb, int& end) {
+    if constexpr (SPAN) {
+      const int b = (step * a.slots + slot) * KG + g;
+      wk.block(b, kb, end);
+      return b < wk.nb;
+    } else {
+      kb = (step * KG + g) * kBlk;
+      end = ctx;
+      return kb < ctx;
+    }
+  };
 
   const bool cap = a.softcap > 0.f;
   float qv[NC][8];
   float amax = 0.f;
   {
-    const float* qp = a.q + (size_t)min(z, a.n_tok - 1) * a.tok_q + ((size_t)kvh * G + hq) * HD + 8 * h;
+    const float* qp = a.q + (size_t)min(z, a.n_tok - 1) * a.tok_q + head_at(hq) + 8 * h;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const float4 x0 = *reinterpret_cast<const float4*>(qp + 16 * (ds * NC + c));
@@ -212,15 +273,15 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
   // this group's block of a step -> LDS, each of its RT * DS waves a share
   // (positions past ctx - 1 reload ctx - 1: finite, masked)
   auto stage = [&](int step, v4u* kd, v4u* vd) {
-    const int kb = (step * KG + g) * kBlk;
-    if (kb >= ctx) return;
+    int kb, end;
+    if (!block(step, kb, end)) return;
     int ln = lane;
     if (HD == 256) asm volatile("" : "+v"(ln));   // places computed again each step, not kept in registers
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       const int base = ((rt * DS + ds) * kLoads + k) * 64;
       const int r = (base + ln) / CH, slot = (base + ln) % CH;
-      const int pk = min(kb + tile_key(r), ctx - 1);
+      const int pk = min(kb + tile_key(r), end - 1);
       __builtin_amdgcn_global_load_lds((gbl_ptr_t)(kc + (size_t)pk * HD + 8 * (slot ^ kswz<CH>(r))),
                                        (lds_ptr_t)&kd[g * kGrp + base], 16, 0, 0);
     }
@@ -228,7 +289,7 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
     for (int k = 0; k < kLoads; ++k) {
       const int base = ((rt * DS + ds) * kLoads + k) * 64;
       const int r = (base + ln) / CH, slot = (base + ln) % CH;
-      const int pv = min(kb + r, ctx - 1);
+      const int pv = min(kb + r, end - 1);
       __builtin_amdgcn_global_load_lds((gbl_ptr_t)(vc + (size_t)pv * HD + 8 * (slot ^ vswz<CH>(r))),
                                        (lds_ptr_t)&vd[g * kGrp + base], 16, 0, 0);
     }
@@ -239,21 +300,22 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
   v4u kq[kQLoads], vq[kQLoads];
   float qsc = 0.f;
   auto load_q = [&](int step) {
-    const int kb = (step * KG + g) * kBlk;
-    if (kb >= ctx) return;
+    int kb, end;
+    if (!block(step, kb, end)) return;
     const int8_t* k8 = static_cast<const int8_t*>(a.kc) + head_base;
     const int8_t* v8 = static_cast<const int8_t*>(a.vc) + head_base;
 #pragma unroll
     for (int k = 0; k < kQLoads; ++k) {
       const int i = ((rt * DS + ds) * kQLoads + k) * 64 + lane;
-      const int pk = min(kb + tile_key(i / kQRow), ctx - 1), pv = min(kb + i / kQRow, ctx - 1);
+      const int pk = min(kb + tile_key(i / kQRow), end - 1), pv = min(kb + i / kQRow, end - 1);
       kq[k] = *reinterpret_cast<const v4u*>(k8 + (size_t)pk * HD + 16 * (i % kQRow));
       vq[k] = *reinterpret_cast<const v4u*>(v8 + (size_t)pv * HD + 16 * (i % kQRow));
     }
-    qsc = (h ? a.vs : a.ks)[min(kb + n, ctx - 1)];
+    qsc = (h ? a.vs : a.ks)[min(kb + n, end - 1)];
   };
   auto store_q = [&](int step, v4u* kd, v4u* vd, float (*scd)[64]) {
-    if ((step * KG + g) * kBlk >= ctx) return;
+    int kb, end;
+    if (!block(step, kb, end)) return;
 #pragma unroll
     for (int k = 0; k < kQLoads; ++k) {
       const int i = ((rt * DS + ds) * kQLoads + k) * 64 + lane;
@@ -333,11 +395,15 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
       if (Q8) load_q(st + 1);
       else stage(st + 1, knxt, vnxt);
     }
-    const int kb = (st * KG + g) * kBlk;
+    int kb, end;
+    const bool there = block(st, kb, end);
+    // some row of this wave sees some position of the block
+    bool sees = kb <= wmax;
+    if constexpr (SPAN) sees = sees && there && (kb + kBlk - 1 > wmin - a.s.window || kb < a.s.sinks);
     const v4u* kcur = kall + g * kGrp;
     const v4u* vcur = vall + g * kGrp;
     v16f acc = v16f{};
-    if (kb <= wmax) {
+    if (sees) {
       auto read_k = [&](int c) {
         return __builtin_bit_cast(v8h, kcur[n * CH + ((2 * (ds * NC + c) + h) ^ kswz<CH>(n))]);
       };
@@ -369,7 +435,7 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
 #pragma unroll
       for (int j = 0; j < 16; ++j) acc[j] += xs[wave ^ 1][64 * j + lane];
     }
-    if (kb <= wmax) {
+    if (sees) {
       // element j is key kb + 16(j/8) + 8h + j%8 of row n
       float sc[16];
 #pragma unroll
@@ -383,7 +449,18 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
 #pragma unroll
         for (int j = 0; j < 16; ++j) sc[j] = softcap(sc[j] * qscale, a);
       }
-      if (kb + kBlk - 1 > wmin) {   // causal limit
+      if constexpr (SPAN) {
+        if (kb + kBlk > end || kb + kBlk - 1 > wmin || (kb <= wlow && kb + kBlk > a.s.sinks)) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int key = kb + 16 * (j / 8) + 8 * h + j % 8;
+            if (key >= end || key > lim || (key <= low && key >= a.s.sinks)) {
+              sc[j] = -INFINITY;
+              if constexpr (Q8) vsc[j] = 0.f;
+            }
+          }
+        }
+      } else if (kb + kBlk - 1 > wmin) {   // causal limit
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (kb + 16 * (j / 8) + 8 * h + j % 8 > lim) {
@@ -511,7 +588,8 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
       lt += mk == -INFINITY ? 0.f : gl[k][32 * rt + n] * __builtin_amdgcn_exp2f(mk - mx);
     }
     // (a row whose scores are all -inf keeps its 0 / 0)
-    const float f = (m == -INFINITY ? 0.f : pow2((Q8 ? ex : m) - kPExp - mx)) / lt;
+    // SPAN: the slot's share, at the maximum mx
+    const float f = (m == -INFINITY ? 0.f : pow2((Q8 ? ex : m) - kPExp - (SPAN && mx == -INFINITY ? 0.f : mx))) / (leaves_share(a) ? 1.f : lt);
     auto bank = [&](int w) { return w == 0 ? ks0 : w == 1 ? vs0 : w == 2 ? ks1 : vs1; };
     const int tile = wave / DS;
     float4* dst = reinterpret_cast<float4*>(bank(tile / (KG / 2))) + (tile % (KG / 2)) * (32 * HD / 4);
@@ -526,7 +604,7 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
     float odd = 0.f;   // NaN: some output of this thread is not finite
     for (int i = tid; i < RT * 32 * (HD / 4); i += NT) {
       const int r = i / (HD / 4), c = i % (HD / 4);
-      const int zr = (row0 + r) / G, hr = (row0 + r) % G;
+      const int zr = token(row0 + r), hr = head_of(row0 + r);
       const bool live = zr < a.n_tok;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -539,19 +617,34 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
         s.z += v.z;
         s.w += v.w;
       }
-      if (live) *reinterpret_cast<float4*>(a.out + (size_t)zr * a.tok_o + ((size_t)kvh * G + hr) * HD + 4 * c) = s;
+      if constexpr (SPAN) {
+        if (a.slots > 1) {
+          const int rows = a.s.n * a.n_kv_heads << a.s.gs;
+          const size_t head = row_head(a.s, kvh, row0 + r);
+          if (live) reinterpret_cast<float4*>(slot_part<HD>(a.s, rows, slot) + head * HD)[c] = s;
+          if (live && c == 0) {
+            float mr = -INFINITY, lr = 0.f;
+            for (int k = 0; k < KG; ++k) mr = fmaxf(mr, gm[k][r]);
+            for (int k = 0; k < KG; ++k) lr += gl[k][r] * (gm[k][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(gm[k][r] - mr));
+            slot_ml<HD>(a.s, rows, a.slots, slot)[head] = make_float2(lr != lr ? 0.f : mr, lr);
+          }
+          continue;
+        }
+      }
+      if (live) *reinterpret_cast<float4*>(a.out + (size_t)zr * a.tok_o + head_at(hr) + 4 * c) = s;
+      if constexpr (SPAN) mend_rows<HD, Q8>(a.s, live, s, row_head(a.s, kvh, row0 + r));
       // (inf - inf and NaN - NaN are NaN)
-      if (!Q8 && live) odd += (s.x - s.x) + (s.y - s.y) + (s.z - s.z) + (s.w - s.w);
+      if (!SPAN && !Q8 && live) odd += (s.x - s.x) + (s.y - s.y) + (s.z - s.z) + (s.w - s.w);
     }
     // fp16: rows that are not finite, again, each over the positions it sees
     // alone (layer_scheduler.c:415-468 reads no others). A row's HD / 4 threads
     // are neighbours in one wave.
-    if (!Q8 && __ballot(odd != odd)) {
+    if (!SPAN && !Q8 && __ballot(odd != odd)) {
       vm_drain();   // this wave's stores
 #pragma unroll 1
       for (int i = tid; i < RT * 32 * (HD / 4); i += NT) {
-        const int r = i / (HD / 4), z = (row0 + r) / G;
-        float* op = a.out + (size_t)z * a.tok_o + ((size_t)kvh * G + (row0 + r) % G) * HD;
+        const int r = i / (HD / 4), z = token(row0 + r);
+        float* op = a.out + (size_t)z * a.tok_o + head_at(head_of(row0 + r));
         float d = 0.f;
         if (z < a.n_tok)
           for (int k = 0; k < 4; ++k) d += op[4 * (i % (HD / 4)) + k] - op[4 * (i % (HD / 4)) + k];
@@ -559,8 +652,8 @@ __global__ void __launch_bounds__(RT * KG * DS * 64) k_flash_rows(const AttnArgs
         while (bad) {
           const int at = __ffsll((unsigned long long)bad) - 1, rb = __shfl(r, at, kWave);
           bad &= ~(((HD / 4 < 64 ? 1ull << (HD / 4 % 64) : 0ull) - 1) << (at / (HD / 4) * (HD / 4)));
-          const int zb = (row0 + rb) / G;
-          const size_t head = ((size_t)kvh * G + (row0 + rb) % G) * HD;
+          const int zb = token(row0 + rb);
+          const size_t head = head_at(head_of(row0 + rb));
           one_row<HD>(a, a.q + (size_t)zb * a.tok_q + head, kc, vc, a.pos0 + zb, a.out + (size_t)zb * a.tok_o + head);
         }
       }

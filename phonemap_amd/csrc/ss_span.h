@@ -127,4 +127,55 @@ __device__ __forceinline__ void span_row(const SpanArgs& a, const float* q, floa
   for (int i = 0; i < ND; ++i) out[lane + kWave * i] = none ? 0.f : o[i] / l;
 }
 
+constexpr int kKeys = 32;   // keys per block
+__device__ __forceinline__ int blocks_of(int n) { return (n + kKeys - 1) / kKeys; }
+
+// What a tile of rows walks: blocks of positions [0, to0), then of [from1, to1), of one KV head's K and V.
+struct Walk {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  int to0, from1, to1;
+  int nb0, nb;   // blocks of the first span, of both
+  __device__ __forceinline__ void block(int b, int& key, int& limit) const {
+    key = b < nb0 ? kKeys * b : from1 + kKeys * (b - nb0);
+    limit = b < nb0 ? to0 : to1;
+  }
+};
+
+// among all rows [n][n_heads]
+__device__ __forceinline__ size_t row_head(const SpanArgs& a, int kvh, int row) {
+  return ((size_t)(row >> a.gs) * a.n_kv_heads + kvh << a.gs) + (row & ((1 << a.gs) - 1));
+}
+
+// slot s of row `head` of all rows: part [slots][rows][HD], then (m, l) [slots][rows]
+template <int HD>
+__device__ __forceinline__ float* slot_part(const SpanArgs& a, int rows, int s) { return a.part + (size_t)s * rows * HD; }
+template <int HD>
+__device__ __forceinline__ float2* slot_ml(const SpanArgs& a, int rows, int slots, int s) {
+  return reinterpret_cast<float2*>(a.part + (size_t)slots * rows * HD) + (size_t)s * rows;
+}
+
+// One row in fp32 where the products could not serve it: a V that is not finite
+// reaches, as 0 * inf, rows of the tile that do not see its position, and meets
+// two parts of a weight where it is one. Whole waves, rows of HD / 4
+// neighbouring lanes: s is this lane's share of row `head`.
+template <int HD, int KVT>
+__device__ __forceinline__ void mend_rows(const SpanArgs& a, bool live, float4 s, size_t head) {
+  const float odd = live ? (s.x - s.x) + (s.y - s.y) + (s.z - s.z) + (s.w - s.w) : 0.f;   // NaN: something is not finite
+  uint64_t bad = __ballot(odd != odd);
+  if (!bad) return;
+  vm_drain();   // this wave's stores
+  const int nh = a.n_kv_heads << a.gs;
+  while (bad) {
+    const int at = __ffsll((unsigned long long)bad) - 1;
+    const int row = __shfl((int)head, at, kWave);
+    bad &= ~(((HD / 4 < 64 ? 1ull << (HD / 4 % 64) : 0ull) - 1) << (at / (HD / 4) * (HD / 4)));
+    Span sp[2];
+    row_spans<HD, KVT>(a, row / nh, row % nh >> a.gs, sp);
+    span_row<HD, KVT>(a, a.q + (size_t)row * HD, a.out + (size_t)row * HD, sp);
+  }
+}
+
 }  // namespace ssk

@@ -36,8 +36,6 @@
 namespace ssk {
 namespace {
 
-constexpr int kKeys = 32;   // keys per block
-
 // value of the lane 16 away (lane ^ 16) joined to this one's
 __device__ __forceinline__ float max_16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -47,30 +45,31 @@ __device__ __forceinline__ float sum_16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ float swap_8(float v) { return dpp<0x128>(v); }   // row_ror:8: lane ^ 8
-
-// What a tile of rows walks: blocks of positions [0, to0), then of [from1, to1), of one KV head's K and V.
-struct Walk {
-  const uint8_t* k;
-  const uint8_t* v;
-  const float* ks;
-  const float* vs;
-  int to0, from1, to1;
-  int nb0, nb;   // blocks of the first span, of both
-  __device__ __forceinline__ void block(int b, int& key, int& limit) const {
-    key = b < nb0 ? kKeys * b : from1 + kKeys * (b - nb0);
-    limit = b < nb0 ? to0 : to1;
-  }
-};
+__device__ __forceinline__ float swap_8(float v) {   // row_ror:8: lane ^ 8
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x128, 0xf, 0xf, true));
+}
+// a barrier for what is in LDS: loads from memory stay in flight
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// maximum over aligned groups of N lanes
+template <int N>
+__device__ __forceinline__ float max_lanes(float v) {
+  static_assert(N == 8 || N == 16 || N == 32, "");
+  v = fmaxf(v, dpp<0xb1>(v));
+  v = fmaxf(v, dpp<0x4e>(v));
+  v = fmaxf(v, dpp<0x141>(v));
+  if constexpr (N >= 16) v = fmaxf(v, dpp<0x140>(v));
+  if constexpr (N >= 32) v = max_16(v);
+  return v;
+}
 
 // The tile's rows: row r is query head g of token or sequence t, t * G + g = r0 + r < r1.
 struct Rows {
   int r0, r1, kvh;
 };
-// among all rows [n][n_heads]
-__device__ __forceinline__ size_t row_head(const SpanArgs& a, int kvh, int row) {
-  return ((size_t)(row >> a.gs) * a.n_kv_heads + kvh << a.gs) + (row & ((1 << a.gs) - 1));
-}
 
 // One block's K and V of a wave
 template <int HD, int KVT>
@@ -162,109 +161,119 @@ __device__ __forceinline__ int slice_dim(int c, int kq) {
 }
 
 __host__ __device__ constexpr int tile_rows(int rt) { return rt == 0 ? 8 : 16 * rt; }
-// waves of a workgroup, and at most that many per SIMD by their registers
-__host__ __device__ constexpr int tile_waves(int hd, int rt) { return rt == 0 && hd < 256 ? 8 : 4; }
+constexpr int kW = 4;   // waves of a workgroup
+// and at most that many per SIMD, by their registers
 __host__ __device__ constexpr int simd_waves(int hd) { return hd < 256 ? 2 : 1; }
 
-template <int HD, int RT, int W>
-struct Joint {   // the results of W waves
-  static constexpr int kPitch = HD + 4;
-  float o[W][tile_rows(RT)][kPitch];
-  float m[W][tile_rows(RT)], l[W][tile_rows(RT)], e[W][tile_rows(RT)];
+// A workgroup's LDS: first q, its parts as rows (n and rows + n) in the order of
+// the products' operand; then the waves' results.
+template <int HD, int RT>
+union Joint {
+  static constexpr int kRows = tile_rows(RT);
+  struct {
+    _Float16 part[2 * kRows][HD + 8];
+    float scale[kRows];
+  } q;
+  struct {
+    float o[kW][kRows][HD + 4];
+    float m[kW][kRows], l[kW][kRows], e[kW][kRows];
+  } r;
 };
 
-// One row in fp32 where the products could not serve it: a V that is not finite
-// reaches, as 0 * inf, rows of the tile that do not see its position. Whole
-// waves, rows of HD / 4 neighbouring lanes: s is this lane's share of row `head`.
-template <int HD>
-__device__ __forceinline__ void mend_rows(const SpanArgs& a, bool live, float4 s, size_t head) {
-  const float odd = live ? (s.x - s.x) + (s.y - s.y) + (s.z - s.z) + (s.w - s.w) : 0.f;   // NaN: something is not finite
-  uint64_t bad = __ballot(odd != odd);
-  if (!bad) return;
-  vm_drain();   // this wave's stores
-  const int nh = a.n_kv_heads << a.gs;
-  while (bad) {
-    const int at = __ffsll((unsigned long long)bad) - 1;
-    const int row = __shfl((int)head, at, kWave);
-    bad &= ~(((HD / 4 < 64 ? 1ull << (HD / 4 % 64) : 0ull) - 1) << (at / (HD / 4) * (HD / 4)));
-    Span sp[2];
-    row_spans<HD, 0>(a, row / nh, row % nh >> a.gs, sp);
-    span_row<HD, 0>(a, a.q + (size_t)row * HD, a.out + (size_t)row * HD, sp);
-  }
-}
-
-// A tile of rows over the walk's blocks b with b / W % slots == slot, by W waves:
-// the rows' outputs (part null), or the slot's share of them, at part[row of
-// all rows][HD] and ml[row], to be joined. RT 0: 8 rows or fewer in one product;
-// else RT tiles of 16.
-template <int HD, int KVT, int RT, int W, class Masks>
+// A tile of rows over the walk's blocks b with b / kW % slots == slot, by the
+// workgroup's waves: the rows' outputs (part null), or the slot's share of them,
+// at part[row of all rows][HD] and ml[row], to be joined. RT 0: 8 rows or fewer
+// in one product; else RT tiles of 16.
+template <int HD, int KVT, int RT, class Masks>
 __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, const Walk& w, int slot, int slots, float* part,
-                                          float2* ml, Joint<HD, RT, W>& sh, Masks masks) {
+                                          float2* ml, Joint<HD, RT>& sh, Masks masks) {
   constexpr bool PACK = RT == 0;
-  constexpr int NT = PACK ? 1 : RT, NC = HD / 32, DPL = HD / 16;
+  constexpr int kRows = tile_rows(RT), NT = PACK ? 1 : RT, NC = HD / 32, DPL = HD / 16;
   using Blk = Block<HD, KVT>;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, kq = lane >> 4;
-  const int b0 = slot * W + wave, step = slots * W;
+  const int b0 = slot * kW + wave, step = slots * kW;
+  const bool cap = a.softcap > 0.f;
 
+  // the tile's q, 8 values a thread, requested ahead of the first block
+  constexpr int kChunks = kRows * HD / 8, kTurns = (kChunks + kW * 64 - 1) / (kW * 64);
+  static_assert(kChunks % 64 == 0, "whole waves");
+  float qv[kTurns][8];
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int i = tid + u * kW * 64, row = rows.r0 + i / (HD / 8);
+    if (i < kChunks) {
+      const float* qp = a.q + row_head(a, rows.kvh, min(row, rows.r1 - 1)) * HD + i % (HD / 8) * 8;
+      const float4 x0 = *reinterpret_cast<const float4*>(qp), x1 = *reinterpret_cast<const float4*>(qp + 4);
+      qv[u][0] = x0.x, qv[u][1] = x0.y, qv[u][2] = x0.z, qv[u][3] = x0.w;
+      qv[u][4] = x1.x, qv[u][5] = x1.y, qv[u][6] = x1.z, qv[u][7] = x1.w;
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  // (a wave without a block, or past its last, loads from an empty view: no
+  // branch, so a wait counts the loads behind the one it is for)
   Blk blk;
   int key = 0, limit = 0;
-  if (b0 < w.nb) {
-    w.block(b0, key, limit);
-    blk.load_k(w, key, limit, n, kq);
-    blk.load_v(w, key, limit, n, kq);
-  }
+  auto next = [&](int b) {
+    w.block(b, key, limit);
+    if (b >= w.nb) key = limit = 0;
+  };
+  next(b0);
+  blk.load_k(w, key, limit, n, kq);
+  blk.load_v(w, key, limit, n, kq);
+  __builtin_amdgcn_sched_barrier(0);
 
-  // q of row n of each tile as B: times the softmax's scale and log2 e, its
-  // largest magnitude brought to [2^13, 2^14), in two parts
+  // q times the softmax's scale and log2 e, a row's largest magnitude brought to
+  // [2^13, 2^14), in two parts
+#pragma unroll
+  for (int u = 0; u < kTurns; ++u) {
+    const int i = tid + u * kW * 64, r = i / (HD / 8), c = i % (HD / 8);
+    if (i < kChunks) {
+      const bool live = rows.r0 + r < rows.r1;
+      float amax = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        qv[u][k] = live ? qv[u][k] : 0.f;
+        amax = fmaxf(amax, fabsf(qv[u][k]));
+      }
+      amax = max_lanes<HD / 8>(amax);
+      int e = 0;
+      const float c0 = cap ? a.scale : a.scale * kLog2e;
+      const float c1 = cap ? 0.f : __builtin_fmaf(a.scale, kLog2e, -c0) + a.scale * kLog2eLow;
+      frexpf(amax * c0, &e);
+      const int shift = min(max(14 - e, -100), 100);
+      const float s0 = ldexpf(c0, shift), s1 = ldexpf(c1, shift);
+      if (c == 0) sh.q.scale[r] = ldexpf(1.0f, -shift);   // S^T holds the scores * 2^shift
+      v8h hi, lo;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float p = qv[u][k] * s0;
+        asm("" : "+v"(p));   // one value for both parts
+        hi[k] = (_Float16)p;
+        lo[k] = (_Float16)__builtin_fmaf(qv[u][k], s1, __builtin_fmaf(qv[u][k], s0, -(float)hi[k]));
+      }
+      *reinterpret_cast<v8h*>(&sh.q.part[r][8 * c]) = hi;
+      *reinterpret_cast<v8h*>(&sh.q.part[kRows + r][8 * c]) = lo;
+    }
+  }
+  lds_barrier();
+  // row n of each tile as B (PACK: rows 8 .. 15 are the low parts)
   v8h qh[NT][NC], ql[PACK ? 1 : NT][PACK ? 1 : NC];
   float qscale[NT];
   int row[NT];
-  const bool cap = a.softcap > 0.f;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    row[t] = rows.r0 + (PACK ? n & 7 : 16 * t + n);
-    const bool live = row[t] < rows.r1;
-    const int at = min(row[t], rows.r1 - 1);
-    const float* qp = a.q + row_head(a, rows.kvh, at) * HD;
-    float qv[NC][8], amax = 0.f;
+    const int r = PACK ? n & 7 : 16 * t + n;
+    row[t] = rows.r0 + r;
+    qscale[t] = sh.q.scale[r];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const float4 x0 = *reinterpret_cast<const float4*>(qp + slice_dim<KVT>(c, kq));
-      const float4 x1 = *reinterpret_cast<const float4*>(qp + slice_dim<KVT>(c, kq) + 4);
-      qv[c][0] = x0.x, qv[c][1] = x0.y, qv[c][2] = x0.z, qv[c][3] = x0.w;
-      qv[c][4] = x1.x, qv[c][5] = x1.y, qv[c][6] = x1.z, qv[c][7] = x1.w;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        qv[c][i] = live ? qv[c][i] : 0.f;
-        amax = fmaxf(amax, fabsf(qv[c][i]));
-      }
+      qh[t][c] = *reinterpret_cast<const v8h*>(&sh.q.part[PACK ? n : r][slice_dim<KVT>(c, kq)]);
+      if constexpr (!PACK) ql[t][c] = *reinterpret_cast<const v8h*>(&sh.q.part[kRows + r][slice_dim<KVT>(c, kq)]);
     }
-    amax = max_pair(max_16(amax));
-    int e = 0;
-    const float c0 = cap ? a.scale : a.scale * kLog2e;
-    const float c1 = cap ? 0.f : __builtin_fmaf(a.scale, kLog2e, -c0) + a.scale * kLog2eLow;
-    frexpf(amax * c0, &e);
-    const int shift = min(max(14 - e, -100), 100);
-    const float sh0 = ldexpf(c0, shift), sh1 = ldexpf(c1, shift);
-    qscale[t] = ldexpf(1.0f, -shift);   // S^T holds the scores * 2^shift
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float p = qv[c][i] * sh0;
-        asm("" : "+v"(p));   // one value for both parts
-        const _Float16 hi = (_Float16)p;
-        const _Float16 lo = (_Float16)__builtin_fmaf(qv[c][i], sh1, __builtin_fmaf(qv[c][i], sh0, -(float)hi));
-        if constexpr (PACK) {
-          qh[t][c][i] = n < 8 ? hi : lo;
-        } else {
-          qh[t][c][i] = hi;
-          ql[t][c][i] = lo;
-        }
-      }
   }
+  lds_barrier();   // (the waves' results take q's place)
 
   v4f o[NT][DPL];
   float m[NT], l[NT], ex[NT];   // running maximum, this lane's share of the sum; int8: O's exponent, times 2^12
@@ -301,10 +310,8 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
     }
     const int at = key, end = limit;
     __builtin_amdgcn_sched_barrier(0);
-    if (b + step < w.nb) {
-      w.block(b + step, key, limit);
-      blk.load_k(w, key, limit, n, kq);
-    }
+    next(b + step);
+    blk.load_k(w, key, limit, n, kq);
     __builtin_amdgcn_sched_barrier(0);
 
     v8h ph[NT], pl[PACK ? 1 : NT];
@@ -332,7 +339,7 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
         const float mn = ceilf(fmaxf(m[t], bmax));
         const float corr = pow2(m[t] - (mn == -INFINITY ? 0.f : mn));
         l[t] *= corr;
-        if constexpr (KVT == 0) {
+        if (KVT == 0 && b != b0) {   // (nothing there yet)
 #pragma unroll
           for (int j = 0; j < DPL; ++j) o[t][j] *= corr;
         }
@@ -388,7 +395,7 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (b + step < w.nb) blk.load_v(w, key, limit, n, kq);
+    blk.load_v(w, key, limit, n, kq);
     __builtin_amdgcn_sched_barrier(0);
   }
 
@@ -405,11 +412,11 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
     const int at = PACK ? n & 7 : 16 * t + n;
     if (!PACK || n < 8) {
       if (kq == 0) {
-        sh.m[wave][at] = m[t];
-        sh.l[wave][at] = l[t];
-        sh.e[wave][at] = KVT == 1 ? ex[t] : m[t];
+        sh.r.m[wave][at] = m[t];
+        sh.r.l[wave][at] = l[t];
+        sh.r.e[wave][at] = KVT == 1 ? ex[t] : m[t];
       }
-      float* dst = &sh.o[wave][at][4 * DPL * kq];
+      float* dst = &sh.r.o[wave][at][4 * DPL * kq];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -419,20 +426,20 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
   }
   __syncthreads();
   constexpr int kQuads = HD / 4;
-  static_assert(tile_rows(RT) * kQuads % (W * 64) == 0 || tile_rows(RT) * kQuads < W * 64, "whole waves");
-  for (int i = tid; i < tile_rows(RT) * kQuads; i += W * 64) {
+  static_assert(kRows * kQuads % 64 == 0, "whole waves");
+  for (int i = tid; i < kRows * kQuads; i += kW * 64) {
     const int r = i / kQuads, c = i % kQuads, all = rows.r0 + r;
     const bool live = all < rows.r1;
     float mx = -INFINITY, lt = 0.f;
 #pragma unroll
-    for (int k = 0; k < W; ++k) mx = fmaxf(mx, sh.m[k][r]);
+    for (int k = 0; k < kW; ++k) mx = fmaxf(mx, sh.r.m[k][r]);
     const float mo = mx == -INFINITY ? 0.f : mx;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      lt += sh.l[k][r] * pow2(sh.m[k][r] - mo);
-      const float f = pow2(sh.e[k][r] - kPExp - mo);
-      const float4 v = *reinterpret_cast<const float4*>(&sh.o[k][r][4 * c]);
+    for (int k = 0; k < kW; ++k) {
+      lt += sh.r.l[k][r] * pow2(sh.r.m[k][r] - mo);
+      const float f = pow2(sh.r.e[k][r] - kPExp - mo);
+      const float4 v = *reinterpret_cast<const float4*>(&sh.r.o[k][r][4 * c]);
       s.x += v.x * f;
       s.y += v.y * f;
       s.z += v.z * f;
@@ -448,14 +455,13 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
       const float f = w.nb == 0 ? 0.f : 1.f / lt;   // no position at all: 0
       s = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
       if (live) reinterpret_cast<float4*>(a.out + head * HD)[c] = s;
-      if constexpr (KVT == 0 && Masks::kMend) mend_rows<HD>(a, live, s, head);
+      mend_rows<HD, KVT>(a, live, s, head);
     }
   }
 }
 
 // Keys at or past the block's end are not there.
 struct TailMask {
-  static constexpr bool kMend = false;
   template <class F>
   __device__ __forceinline__ void apply(int key, int limit, int kq, int row, F hide) const {
     if (key + kKeys > limit) {
@@ -467,7 +473,6 @@ struct TailMask {
 };
 // Rows of several tokens: row r's token sees its own window alone.
 struct WindowMask {
-  static constexpr bool kMend = true;
   int gs, pos0, window, sinks, t0, t1;   // the tile's first and last token
   template <class F>
   __device__ __forceinline__ void apply(int key, int limit, int kq, int row, F hide) const {
@@ -481,20 +486,10 @@ struct WindowMask {
   }
 };
 
-__device__ __forceinline__ int blocks_of(int n) { return (n + kKeys - 1) / kKeys; }
-
-// slot s of row `head` of all rows: part [slots][rows][HD], then (m, l) [slots][rows]
-template <int HD>
-__device__ __forceinline__ float* slot_part(const SpanArgs& a, int rows, int s) { return a.part + (size_t)s * rows * HD; }
-template <int HD>
-__device__ __forceinline__ float2* slot_ml(const SpanArgs& a, int rows, int slots, int s) {
-  return reinterpret_cast<float2*>(a.part + (size_t)slots * rows * HD) + (size_t)s * rows;
-}
-
 // Grid: n_kv_heads x slots.
 template <int HD, int KVT, int RT>
-__global__ void __launch_bounds__(tile_waves(HD, RT) * 64, simd_waves(HD)) k_span_window(const SpanArgs a, int slots) {
-  __shared__ Joint<HD, RT, tile_waves(HD, RT)> sh;
+__global__ void __launch_bounds__(kW * 64, simd_waves(HD)) k_span_window(const SpanArgs a, int slots) {
+  __shared__ Joint<HD, RT> sh;
   const int kvh = blockIdx.x % a.n_kv_heads, slot = blockIdx.x / a.n_kv_heads;
   const int end = a.pos0 + a.n, rows = a.n * a.n_kv_heads << a.gs;
   Walk w;
@@ -520,10 +515,10 @@ __global__ void __launch_bounds__(tile_waves(HD, RT) * 64, simd_waves(HD)) k_spa
 // Grid: n_kv_heads x np x tiles of rows over the prefix, then n_kv_heads x no x
 // sequences over their own caches; slots 0 .. np - 1 are the prefix's.
 template <int HD, int KVT, int RT>
-__global__ void __launch_bounds__(tile_waves(HD, RT) * 64, simd_waves(HD)) k_span_shared(const SpanArgs a, int np, int no, int tiles) {
+__global__ void __launch_bounds__(kW * 64, simd_waves(HD)) k_span_shared(const SpanArgs a, int np, int no, int tiles) {
   __shared__ union {
-    Joint<HD, RT, tile_waves(HD, RT)> tile;
-    Joint<HD, 0, tile_waves(HD, RT)> own;
+    Joint<HD, RT> tile;
+    Joint<HD, 0> own;
   } sh;
   const int slots = np + no, rows = a.n * a.n_kv_heads << a.gs;
   int i = blockIdx.x;
@@ -560,124 +555,136 @@ __global__ void __launch_bounds__(tile_waves(HD, RT) * 64, simd_waves(HD)) k_spa
   }
 }
 
-// The slots' shares -> outputs; one thread per four outputs.
+// The slots' shares -> outputs: a thread takes four outputs of a row from every
+// `groups`-th slot, and the groups of a row meet in LDS.
 constexpr int kJoinThreads = 256;
 template <int HD, int KVT>
-__global__ void __launch_bounds__(kJoinThreads) k_span_join(const SpanArgs a, int slots) {
+__global__ void __launch_bounds__(kJoinThreads) k_span_join(const SpanArgs a, int slots, int groups) {
   constexpr int kQuads = HD / 4;
+  __shared__ float4 so[kJoinThreads];
+  __shared__ float2 sml[kJoinThreads];
+  const int tid = threadIdx.x, c = tid % kQuads, g = tid / kQuads % groups;
   const int rows = a.n * a.n_kv_heads << a.gs;
-  const int at = (int)(((int64_t)blockIdx.x * kJoinThreads + threadIdx.x) / kQuads), c = threadIdx.x % kQuads;
+  const int64_t at = (int64_t)blockIdx.x * (kJoinThreads / kQuads / groups) + tid / kQuads / groups;
   const bool live = at < rows;
-  const int row = min(at, rows - 1);
+  const int row = live ? (int)at : rows - 1;
   const float2* ml = slot_ml<HD>(a, rows, slots, 0) + row;
-  float mx = -INFINITY;
-#pragma unroll 8
-  for (int s = 0; s < slots; ++s) mx = fmaxf(mx, ml[(size_t)s * rows].x);
-  float lt = 0.f;
+  const float4* part = reinterpret_cast<const float4*>(a.part + (size_t)row * HD) + c;
+  float mx = -INFINITY, lt = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < slots; ++s) {
-    const float2 x = ml[(size_t)s * rows];
-    if (x.x == -INFINITY) continue;
-    const float4 v = reinterpret_cast<const float4*>(slot_part<HD>(a, rows, s) + (size_t)row * HD)[c];
-    const float f = pow2(x.x - mx);
-    lt += x.y * f;
-    o.x += v.x * f;
-    o.y += v.y * f;
-    o.z += v.z * f;
-    o.w += v.w * f;
+  auto add = [&](float2 x, float4 v) {   // (m, l) and values held relative to m
+    const float mn = fmaxf(mx, x.x), mo = mn == -INFINITY ? 0.f : mn;
+    const float f0 = pow2(mx - mo), f1 = pow2(x.x - mo);
+    lt = lt * f0 + x.y * f1;
+    o = make_float4(o.x * f0 + v.x * f1, o.y * f0 + v.y * f1, o.z * f0 + v.z * f1, o.w * f0 + v.w * f1);
+    mx = mn;
+  };
+  for (int s0 = g; s0 < slots; s0 += 4 * groups) {
+    float2 x[4];
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {   // (past the last: the last again, not added)
+      const int s = min(s0 + k * groups, slots - 1);
+      x[k] = ml[(size_t)s * rows];
+      v[k] = part[(size_t)s * rows * kQuads];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (s0 + k * groups < slots) add(x[k], v[k]);
   }
+  if (groups > 1) {
+    so[tid] = o;
+    sml[tid] = make_float2(mx, lt);
+    __syncthreads();
+    if (g == 0)
+      for (int k = 1; k < groups; ++k) add(sml[tid + k * kQuads], so[tid + k * kQuads]);
+  }
+  const bool store = live && g == 0;
   bool none = false;
   if (a.own_len) none = a.prefix == 0 && own_length(a, row / (a.n_kv_heads << a.gs)) == 0;
   const float f = none ? 0.f : 1.f / lt;
   o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-  if (live) reinterpret_cast<float4*>(a.out + (size_t)row * HD)[c] = o;
-  if constexpr (KVT == 0)
-    if (!a.own_len && a.n > 1) mend_rows<HD>(a, live, o, (size_t)row);
-}
-
-// ---- many rows: one wave per row and query head -------------------------------
-constexpr int kRowWaves = 4;
-template <int HD, int KVT>
-__global__ void __launch_bounds__(kRowWaves * 64) k_span_rows(const SpanArgs a) {
-  const int nh = a.n_kv_heads << a.gs;
-  const int64_t row = (int64_t)blockIdx.x * kRowWaves + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.n * nh) return;
-  const int t = (int)(row / nh), h = (int)(row % nh);
-  Span s[2];
-  row_spans<HD, KVT>(a, t, h >> a.gs, s);
-  span_row<HD, KVT>(a, a.q + (size_t)row * HD, a.out + (size_t)row * HD, s);
+  if (store) reinterpret_cast<float4*>(a.out + (size_t)row * HD)[c] = o;
+  mend_rows<HD, KVT>(a, store, o, (size_t)row);
 }
 
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // How a call is cut: rt (tile_rows), tiles of rows, slots of the window or the
-// prefix (np) and of the own caches (no). rt -1: too many rows, k_span_rows.
+// prefix (np) and of the own caches (no). A window's rt -1: more rows than a
+// decode step's, for ss_flash_span.hip.
 struct Plan {
   int rt, tiles, np, no;
 };
 int rt_of(int hd, int rows) { return rows <= 8 ? 0 : rows <= 16 || hd == 256 ? 1 : 2; }
 
-// keys: the positions that the window's rows see between them (at most)
+// first, rest: the positions of the two spans that the window's rows see between them
 Plan plan_window(int hd, int group, int n_kv_heads, int n, int64_t first, int64_t rest, int n_cu) {
-  if ((int64_t)n * group > (hd == 256 ? 16 : 32)) return {-1, 1, 1, 0};
-  Plan p;
-  p.rt = rt_of(hd, n * group);
-  p.tiles = 1;
-  p.no = 0;
-  const int64_t nb = (first + kKeys - 1) / kKeys + (rest + kKeys - 1) / kKeys;
-  const int w = tile_waves(hd, p.rt), most = up(n_cu, n_kv_heads);
-  const int64_t want = (nb + w - 1) / w;
+  const int64_t rows = (int64_t)n * group, nb = (first + kKeys - 1) / kKeys + (rest + kKeys - 1) / kKeys;
+  Plan p = {rt_of(hd, (int)rows), 1, 1, 0};
+  if (rows > tile_rows(p.rt)) {
+    p.rt = -1;
+    flash_span_shape(hd, (int)rows, n_kv_heads, nb, n_cu, p.tiles, p.np);
+    return p;
+  }
+  // A block per wave, up to two workgroups per compute unit; up to three blocks
+  // per wave one workgroup does without the join (32 heads on 8, head_dim 128: 9
+  // blocks 5.9 us, in three slots 7.6; 33 blocks 12.3 us, in nine slots 7.9).
+  const int64_t want = nb <= 3 * kW ? 1 : (nb + kW - 1) / kW, most = up(2 * n_cu, n_kv_heads);
   p.np = (int)(want < most ? want : most);
   return p;
 }
 Plan plan_shared(int hd, int group, int n_kv_heads, int n, int prefix, int own_max, int n_cu) {
+  const int rows = n * group, nbp = up(prefix, kKeys), nbo = up(own_max, kKeys);
   Plan p;
-  const int rows = n * group;
   p.rt = prefix ? rt_of(hd, rows) : 0;
   p.tiles = prefix ? up(rows, tile_rows(p.rt)) : 0;
-  const int w = tile_waves(hd, p.rt);
-  const int64_t nbp = up(prefix, kKeys), nbo = up(own_max, kKeys);
-  const int64_t all = (nbp * p.tiles + nbo * n) * n_kv_heads;
-  const int each = up(all, (int64_t)n_cu * 8);   // blocks per wave
-  p.np = up(nbp, (int64_t)w * each);
-  p.no = up(nbo, (int64_t)w * each);
+  const int64_t all = ((int64_t)nbp * p.tiles + (int64_t)nbo * n) * n_kv_heads;
+  const int each = up(all, (int64_t)n_cu * 2 * kW);   // blocks per wave
+  p.np = up(nbp, (int64_t)kW * each);
+  p.no = up(nbo, (int64_t)kW * each);
   return p;
 }
 size_t plan_bytes(const Plan& p, int head_dim, int64_t rows) {
   const int slots = p.np + p.no;
-  return p.rt < 0 || slots < 2 ? 0 : (size_t)slots * rows * (head_dim + 2) * sizeof(float);
+  return slots < 2 ? 0 : (size_t)slots * rows * (head_dim + 2) * sizeof(float);
 }
 
 template <int HD, int KVT>
 hipError_t launch_join(const SpanArgs& a, int slots, hipStream_t s) {
-  const int64_t threads = ((int64_t)a.n * a.n_kv_heads << a.gs) * (HD / 4);
-  hipLaunchKernelGGL((k_span_join<HD, KVT>), dim3((unsigned)up(threads, kJoinThreads)), dim3(kJoinThreads), 0, s, a, slots);
+  int groups = 1;   // a power of two
+  while (groups < kJoinThreads / (HD / 4) && groups * 2 < slots) groups *= 2;
+  const int64_t rows = (int64_t)a.n * a.n_kv_heads << a.gs;
+  const dim3 grid((unsigned)up(rows, kJoinThreads / (HD / 4) / groups));
+  hipLaunchKernelGGL((k_span_join<HD, KVT>), grid, dim3(kJoinThreads), 0, s, a, slots, groups);
   return hipGetLastError();
 }
 
 template <int HD, int KVT, int RT>
 hipError_t launch_rt(const SpanArgs& a, const Plan& p, hipStream_t s) {
-  const dim3 block(tile_waves(HD, RT) * 64);
+  const dim3 block(kW * 64);
   const int64_t wgs = (int64_t)a.n_kv_heads * (a.own_len ? (int64_t)p.np * p.tiles + (int64_t)p.no * a.n : p.np);
   if (wgs > INT32_MAX) return hipErrorInvalidValue;
   if (a.own_len)
     hipLaunchKernelGGL((k_span_shared<HD, KVT, RT>), dim3((unsigned)wgs), block, 0, s, a, p.np, p.no, p.tiles);
   else
     hipLaunchKernelGGL((k_span_window<HD, KVT, RT>), dim3((unsigned)wgs), block, 0, s, a, p.np);
-  const hipError_t e = hipGetLastError();
-  return e != hipSuccess || p.np + p.no < 2 ? e : launch_join<HD, KVT>(a, p.np + p.no, s);
+  return hipGetLastError();
 }
 
 template <int HD, int KVT>
 hipError_t launch_kv(const SpanArgs& a, const Plan& p, hipStream_t s) {
-  if (p.rt == 0) return launch_rt<HD, KVT, 0>(a, p, s);
-  if (p.rt == 1) return launch_rt<HD, KVT, 1>(a, p, s);
-  if constexpr (HD < 256)
-    if (p.rt == 2) return launch_rt<HD, KVT, 2>(a, p, s);
-  const int64_t rows = (int64_t)a.n * a.n_kv_heads << a.gs;
-  hipLaunchKernelGGL((k_span_rows<HD, KVT>), dim3((unsigned)up(rows, kRowWaves)), dim3(kRowWaves * 64), 0, s, a);
-  return hipGetLastError();
+  hipError_t e = hipErrorInvalidValue;
+  if (p.rt < 0) {
+    e = launch_flash_span(HD, KVT, a, p.np, s);
+  } else if (p.rt == 0) {
+    e = launch_rt<HD, KVT, 0>(a, p, s);
+  } else if (p.rt == 1) {
+    e = launch_rt<HD, KVT, 1>(a, p, s);
+  } else if constexpr (HD < 256) {
+    e = launch_rt<HD, KVT, 2>(a, p, s);
+  }
+  return e != hipSuccess || p.np + p.no < 2 ? e : launch_join<HD, KVT>(a, p.np + p.no, s);
 }
 template <int HD>
 hipError_t launch_hd(int kv_type, const SpanArgs& a, const Plan& p, hipStream_t s) {
