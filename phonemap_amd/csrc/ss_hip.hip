@@ -597,10 +597,9 @@ bool span_shape_ok(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_
          ssk::attention_supported(head_dim, n_heads / n_kv_heads) && (int64_t)n * n_heads <= (1 << 24);
 }
 
-int32_t span_scratch(const char* what, ssk::SpanArgs& a, void* ws, size_t have, size_t need) {
+int32_t check_scratch(const char* what, const void* ws, size_t have, size_t need) {
   if (need && (!ws || have < need || !aligned(ws, 16)))
     return fail(kErrParams, "%s: needs a 16-byte aligned workspace of %zu bytes (%zu given)", what, need, ws ? have : (size_t)0);
-  a.part = static_cast<float*>(ws);
   return 0;
 }
 
@@ -774,9 +773,10 @@ int32_t ss_hip_attention_window(ss_hip_ctx_t* c, float* out, const float* q, con
   a.pos0 = pos0;
   a.window = window < max_seq ? window : max_seq;
   a.sinks = n_sinks < max_seq ? n_sinks : max_seq;
-  if (int32_t rc = span_scratch("attention_window", a, ws, ws_bytes,
-                                ss_hip_attention_window_workspace(c, n_heads, n_kv_heads, head_dim, n_tokens, window, n_sinks)))
+  if (int32_t rc = check_scratch("attention_window", ws, ws_bytes,
+                                 ss_hip_attention_window_workspace(c, n_heads, n_kv_heads, head_dim, n_tokens, window, n_sinks)))
     return rc;
+  a.part = static_cast<float*>(ws);
   DeviceScope on(c->device);
   HIP_TRY(on.status);
   HIP_TRY(ssk::launch_span(head_dim, kv_type, a, pick(c, stream)));
@@ -815,9 +815,10 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, con
   a.vos = vs_own;
   a.own_max = own_max;
   a.own_len = own_len;
-  if (int32_t rc = span_scratch("attention_shared", a, ws, ws_bytes,
-                                ss_hip_attention_shared_workspace(c, n_heads, n_kv_heads, head_dim, n_seqs, prefix_len, own_max)))
+  if (int32_t rc = check_scratch("attention_shared", ws, ws_bytes,
+                                 ss_hip_attention_shared_workspace(c, n_heads, n_kv_heads, head_dim, n_seqs, prefix_len, own_max)))
     return rc;
+  a.part = static_cast<float*>(ws);
   DeviceScope on(c->device);
   HIP_TRY(on.status);
   HIP_TRY(ssk::launch_span(head_dim, kv_type, a, pick(c, stream)));
@@ -825,8 +826,8 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, con
 }
 
 size_t ss_hip_sample_rows_workspace(ss_hip_ctx_t* c, int32_t n_rows, int32_t n) {
-  (void)c, (void)n_rows, (void)n;
-  return 0;
+  if (!c || n_rows <= 0 || n_rows > 65535 || n <= 0 || n > ssk::kSampleRowsMaxV) return 0;
+  return ssk::sample_rows_workspace(n_rows, n);
 }
 
 int32_t ss_hip_sample_rows(ss_hip_ctx_t* c, int32_t* out, const float* logits, int32_t n, int32_t n_rows, int64_t ld,
@@ -850,7 +851,8 @@ int32_t ss_hip_sample_rows(ss_hip_ctx_t* c, int32_t* out, const float* logits, i
   a.top_k = top_k > 0 && top_k < n ? top_k : 0;
   a.top_p = top_p > 0.f && top_p < 1.f ? top_p : 1.0;
   a.min_gap = a.temperature > 0.0 && min_p > 0.f ? a.temperature * log((double)min_p) : -INFINITY;
-  (void)ws, (void)ws_bytes;
+  if (int32_t rc = check_scratch("sample_rows", ws, ws_bytes, ssk::sample_rows_workspace(n_rows, n))) return rc;
+  a.work = ws;
   DeviceScope on(c->device);
   HIP_TRY(on.status);
   HIP_TRY(ssk::launch_sample_rows(a, pick(c, stream)));

@@ -54,3 +54,46 @@ def test_shared(bad):
 ], ids=str)
 def test_sample(bad):
     _refused("ss_hip_sample_rows", SAMPLE, **bad)
+
+
+def _context(n_cu=256):
+    """A context's fields as the checks read them: the number of compute units behind device and stream."""
+    ctx = (C.c_uint8 * 4096)()
+    np.frombuffer(ctx, np.int32)[4] = n_cu
+    return ctx
+
+
+@pytest.mark.parametrize("bad", [dict(ws=None), dict(ws=P + 8), dict(ws_bytes=-1)], ids=str)
+def test_workspaces(bad):
+    """None, one that is not aligned, one byte too few."""
+    L, ctx = pm.lib(), _context()
+    x = C.addressof(ctx)
+    needs = [("ss_hip_attention_window", dict(WINDOW, max_seq=5000, pos0=4000, window=3000),
+              L.ss_hip_attention_window_workspace(x, 8, 2, 64, 2, 3000, 1)),
+             ("ss_hip_attention_shared", SHARED, L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2, 20, 10)),
+             ("ss_hip_sample_rows", dict(SAMPLE, n=100000, ld=100000), L.ss_hip_sample_rows_workspace(x, 2, 100000))]
+    for name, good, need in needs:
+        assert need > 0, name
+        _refused(name, good, **dict(dict(ctx=x, ws_bytes=need), **(dict(ws_bytes=need - 1) if "ws_bytes" in bad else bad)))
+        assert str(need) in L.ss_hip_last_error().decode()
+
+
+def test_workspaces_of_refused_shapes():
+    L, ctx = pm.lib(), _context()
+    x = C.addressof(ctx)
+    assert L.ss_hip_attention_window_workspace(None, 8, 2, 64, 2, 3000, 1) == 0
+    assert L.ss_hip_attention_window_workspace(x, 7, 2, 64, 2, 3000, 1) == 0
+    assert L.ss_hip_attention_window_workspace(x, 8, 2, 64, 2 ** 31 - 1, 3000, 1) == 0
+    assert L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2, -1, 10) == 0
+    assert L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2 ** 31 - 1, 10, 10) == 0
+    assert L.ss_hip_sample_rows_workspace(x, 65536, 100000) == 0
+    assert L.ss_hip_sample_rows_workspace(x, 2, 1 << 19) == 0
+
+
+def test_workspaces_cover_every_position():
+    """The window's workspace goes by the window alone: no position asks for more."""
+    L, ctx = pm.lib(), _context()
+    x = C.addressof(ctx)
+    for n in (1, 3, 40):
+        sizes = [L.ss_hip_attention_window_workspace(x, 32, 8, 128, n, w, 4) for w in (1, 10, 100, 1000, 5000, 20000, 2 ** 31 - 1)]
+        assert sizes == sorted(sizes)
