@@ -269,7 +269,8 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t *ctx, float *out_dev, const float *
  * 1); equal logits stay or go together. The token is the first whose running
  * sum of the weights that stay, by index, exceeds u times their sum. top_k and
  * top_p are those of ss_hip_sample_logits, whose sums round to 32 bits where
- * these do not. temperature <= 0: the first maximum. NaN logits count as
+ * these do not; a weight below 2^-45 of the largest counts as none.
+ * temperature <= 0: the first maximum. NaN logits count as
  * -inf; a row without any logit above -inf gives -1. u outside [0, 1) counts
  * as the nearest number inside. */
 size_t ss_hip_sample_rows_workspace(ss_hip_ctx_t *ctx, int32_t n_rows, int32_t n);

@@ -304,9 +304,10 @@ struct SampleRowsArgs {
   double top_p;              // >= 1: off
   double min_gap;            // T * log(min_p): the least x - max that stays (-inf: off)
   void* work;                // sample_rows_workspace() bytes, 8-byte aligned
+  int n_cu;                  // compute units
 };
 constexpr int kSampleRowsMaxV = (1 << 19) - 1;   // sums of weights up to 2^44 stay below 2^63
-size_t sample_rows_workspace(int rows, int V);
+size_t sample_rows_workspace(int rows, int V, int n_cu);
 hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s);
 hipError_t launch_set_state(int* dpos, int* tokens, int pos, int token, hipStream_t s);
 hipError_t launch_advance(int* dpos, hipStream_t s);

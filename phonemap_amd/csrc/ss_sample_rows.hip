@@ -9,23 +9,24 @@
 // the order of the filters does not matter. The token is the first i at which
 // the running sum of the weights that stay exceeds u times their sum.
 //
-// Weights are formed in 64 bits and summed as whole multiples of 2^-44, so no
-// sum depends on the order of its terms and a draw falls to the same entry
-// whatever the split: in 32 bits the running sums of a 128256-entry row are off
-// by some 1e-8, and one row in a thousand would take a neighbouring entry.
+// Weights are formed and summed in 64 bits: in 32 the running sums of a
+// 128256-entry row are off by some 1e-8, and one row in a thousand would take a
+// neighbouring entry. Sums whose terms meet in no fixed order are of whole
+// multiples of 2^-44, so a call gives the same tokens every time.
 //
 // The thresholds come from a histogram over bins of x / T a quarter wide, with
-// the entries and the weights of each: 128 bins from the maximum's down reach
-// e^-31.75, whose weight is 0 (less than half of 2^-44). The highest of the three
-// thresholds lies in one bin; what lies above that bin stays, what lies below
-// goes, and the bin's own entries are gathered and the threshold found among
-// them. A bin with more than kList of them (equal logits), or an x / T past 2^28,
-// leaves the row to `slow`, which selects by the bits of x over the whole row.
+// the number of entries and the weights of each: 128 bins from the maximum's down
+// reach e^-31.75, where all entries together weigh less than 2^-26. The highest
+// of the three thresholds lies in one bin; what lies above that bin stays, what
+// lies below goes, and the bin's own entries are gathered and the threshold found
+// among them. A bin with more than kList of them (equal logits), or |x / T| past
+// 2^18, leaves the row to `slow`, which selects by the bits of x over the whole row.
 //
-// Rows of up to kOneMax entries: one workgroup with the row in registers, one
-// launch. Longer ones: tiles of kTile entries, a launch for their maxima and
-// histograms and a launch that gathers; the row's last workgroup to finish that
-// (an arrival count that the first launch clears) finds threshold and token.
+// Rows of up to kOne entries: one workgroup with the row in registers, one launch.
+// Longer ones: a launch over tiles for their maxima and histograms, and one with a
+// workgroup per row, which adds up the bins, goes through the tiles that have
+// entries in the threshold's bin, and draws within one tile. Weights are formed
+// once, for the histogram, and again for the threshold's bin and the last tile.
 
 #include "ss_device.h"
 #include "ss_kernels.h"
@@ -33,16 +34,17 @@
 namespace ssk {
 namespace {
 
-constexpr double kOne = 17592186044416.0;   // 2^44, the weight of the maximum
+constexpr double kUnit = 17592186044416.0;  // 2^44
 constexpr int kBins = 128;
 constexpr int kCopies = 8;                  // of the histogram, one per lane % 8
-constexpr int kList = 4096;                 // entries of the threshold's bin
-constexpr int kPairs = 160;                 // up to this many are compared each with all
-constexpr int kFar = 1 << 28;               // |bin| this large: not told apart
+constexpr int kList = 8192;                 // entries of the threshold's bin
+constexpr int kPairs = 256;                 // up to this many are compared each with all
+constexpr float kFar = 1048576.f;           // 2^20 bins from 0: neighbours are not told apart
 
-constexpr int kOneThreads = 1024, kOneEach = 32, kOneMax = kOneThreads * kOneEach;
-constexpr int kTileThreads = 512, kTileEach = 16, kTile = kTileThreads * kTileEach;
-constexpr int kMaxTiles = (kSampleRowsMaxV + kTile - 1) / kTile;
+constexpr int kOneThreads = 1024, kOne = 4 * kOneThreads;
+constexpr int kTileThreads = 512;           // of 8 or 16 entries each
+constexpr int kRowThreads = 1024, kRounds = 8;   // the row's workgroup goes through rounds of 4096 entries, 8 at a time
+constexpr int kMaxTiles = (kSampleRowsMaxV + 8 * kTileThreads - 1) / (8 * kTileThreads);   // 128
 
 // unsigned key that orders like the value; NaN as -inf, -0 as 0
 __device__ __forceinline__ uint32_t order(float x) {
@@ -57,33 +59,32 @@ __device__ __forceinline__ float from_order(uint32_t k) {
 __device__ __forceinline__ double gap(float x, float mx) {
   return x == mx ? 0.0 : x == x ? (double)x - (double)mx : -INFINITY;
 }
-__device__ __forceinline__ uint64_t weight(double g, double temperature) {
-  return (uint64_t)(exp(g / temperature) * kOne + 0.5);
-}
-// u * total as a whole multiple, below total; u outside [0, 1) counts as the nearest end
-__device__ __forceinline__ uint64_t draw_target(float u, uint64_t total) {
-  if (!(u > 0.f)) return 0;
-  const uint64_t t = u < 1.f ? (uint64_t)((double)u * (double)total) : total;
-  return t < total ? t : total - 1;
-}
-// the bin of x (4 / T: quarters of x / T), and e^(x / T - the bin's middle) times 2^44
-__device__ __forceinline__ int bin_of(float x, double per) {
-  const double b = x == x ? floor((double)x * per) : -INFINITY;
-  return (int)fmin(fmax(b, (double)-kFar), (double)kFar);
-}
-__device__ __forceinline__ uint64_t bin_weight(float x, double per, int b) {
-  const double r = 0.25 * ((double)x * per - ((double)b + 0.5));   // |r| <= 1/8: the ninth power is below 2e-14
-  double p = 1.0 / 40320;
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return (uint64_t)(p * kOne + 0.5);
-}
+// u as a fraction of 1; u outside [0, 1) counts as the nearest number inside
+__device__ __forceinline__ double fraction(float u) { return u > 0.f ? fmin((double)u, 1.0 - 0x1p-53) : 0.0; }
+
+// The row's scale of bins: 4 / T in 32 bits places x (a rounded product, still in
+// the order of x), 1 / T in 64 bits weighs it.
+struct Scale {
+  float per;
+  double inv;
+  __device__ __forceinline__ float bin(float x) const { return x == x ? floorf(x * per) : -INFINITY; }
+  // e^(x / T - the middle of bin b) in units of 2^-44, for |x / T - that| of 1/8 and a
+  // little: the ninth power's term is below 2e-13
+  __device__ __forceinline__ uint64_t weight(float x, float b) const {
+    const double r = fma((double)x, inv, -0.25 * ((double)b + 0.5));
+    double p = 1.0 / 40320;
+    p = fma(p, r, 1.0 / 5040);
+    p = fma(p, r, 1.0 / 720);
+    p = fma(p, r, 1.0 / 120);
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    // p * 2^44 as a whole number: the low bits of its sum with 2^52 (p is below 2)
+    return (uint64_t)__double_as_longlong(fma(p, kUnit, 0x1p52)) & 0xfffffffffffffull;
+  }
+};
 
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
 #pragma unroll
@@ -136,66 +137,93 @@ __device__ uint64_t sum_before(uint64_t v, uint64_t* red, uint64_t& all) {
   }
   return before;
 }
+// the same of doubles, added in the order of the lanes and waves; red: NT / 64 words
+template <int NT>
+__device__ double group_sum(double v, double* red) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double t = 0.0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) t += red[w];
+  return t;
+}
 __device__ __forceinline__ void add_u64(uint64_t* p, uint64_t v) {
   atomicAdd(reinterpret_cast<unsigned long long*>(p), (unsigned long long)v);
 }
 
-// Selection by the bits of the keys, 8 at a time: the largest key at which the
-// sum of val(i) over the entries i < n with that key or a greater one reaches
-// target, 0 when all together do not. hist: 256 words, red: NT / 64 + 2.
+// Selection by the bits of the keys, kDigit at a time: the largest key at which
+// the sum of val(i) over the entries i < n with that key or a greater one reaches
+// target, 0 when all together do not. hist: 2^kDigit words, red: NT / 64 + 2.
+constexpr int kDigit = 9, kDigits = 1 << kDigit;
 template <int NT, class Key, class Val>
 __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_t* red, Key key, Val val) {
-  uint32_t prefix = 0, mask = 0;
+  static_assert(NT >= kDigits, "a digit per thread");
+  // the bits that all keys share
+  const uint32_t first = key(0);
+  uint32_t differ = 0;
+  for (int i = threadIdx.x; i < n; i += NT) differ |= key(i) ^ first;
+  differ = group_max<NT>(differ ? 32 - __clz((int)differ) : 0, red);   // as many low bits do not
+  int shift = (int)differ;
+  uint32_t mask = shift < 32 ? ~0u << shift : 0u, prefix = first & mask;
   uint64_t above = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
+  do {
+    const int bits = min(kDigit, shift);
+    shift -= bits;
+    const uint32_t digit = (1u << bits) - 1;
     __syncthreads();
-    if (threadIdx.x < 256) hist[threadIdx.x] = 0;
+    if (threadIdx.x < kDigits) hist[threadIdx.x] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += NT) {
       const uint32_t k = key(i);
-      if ((k & mask) == prefix) add_u64(&hist[(k >> shift) & 255u], val(i));
+      if ((k & mask) == prefix) add_u64(&hist[(k >> shift) & digit], val(i));
     }
     __syncthreads();
-    const uint64_t h = threadIdx.x < 256 ? hist[255 - threadIdx.x] : 0;   // thread 0 has the highest digit
+    const uint64_t h = threadIdx.x < kDigits ? hist[kDigits - 1 - threadIdx.x] : 0;   // thread 0 has the highest digit
     uint64_t all;
     const uint64_t before = above + sum_before<NT>(h, red, all);
     uint64_t* found = red + NT / 64;
-    if (threadIdx.x == 0) found[0] = 256;
+    if (threadIdx.x == 0) found[0] = kDigits;
     __syncthreads();
-    if (threadIdx.x < 256 && before < target && before + h >= target) {
-      found[0] = 255 - threadIdx.x;
+    if (threadIdx.x < kDigits && before < target && before + h >= target) {
+      found[0] = kDigits - 1 - threadIdx.x;
       found[1] = before;
     }
     __syncthreads();
-    if (found[0] == 256) return 0;
+    if (found[0] == kDigits) return 0;
     prefix |= (uint32_t)found[0] << shift;
-    mask |= 255u << shift;
+    mask |= digit << shift;
     above = found[1];
-  }
+  } while (shift > 0);
   return prefix;
 }
 
-// What stays, and with which weight.
+// What stays, and with which weight, in units of the middle of the maximum's bin.
 struct Keep {
-  uint32_t least;   // the least key
-  float mx;
-  double temperature, min_gap;
-  __device__ __forceinline__ uint64_t operator()(float x) const {
-    if (order(x) < least) return 0;
-    const double g = gap(x, mx);
-    return g >= min_gap ? weight(g, temperature) : 0;
+  Scale scale;
+  const double* fall;   // e^(-r / 4) of bin top - r
+  float top, mx;
+  double min_gap;
+  uint32_t least;       // the least key
+  __device__ __forceinline__ double operator()(float x) const {
+    const float b = scale.bin(x), r = top - b;
+    if (!(r < kBins) || order(x) < least || !(gap(x, mx) >= min_gap)) return 0.0;
+    return (double)scale.weight(x, b) * fall[(int)r];
   }
 };
 
 // ---- a row's entries in the registers of a workgroup ---------------------------
-// x[4k + j] of thread t is entry i0 + 4 (k * NT + t) + j (-inf past the row)
+// x[4k + j] of thread t is entry 4 (k * NT + t) + j of those loaded (-inf past the row)
 template <int NT, int E>
 struct Chunk {
+  static constexpr int kRounds = E / 4;
   float x[E];
   __device__ __forceinline__ static int at(int k, int j) { return 4 * (k * NT + (int)threadIdx.x) + j; }
   __device__ __forceinline__ void load(const float* row, int i0, int V) {
 #pragma unroll
-    for (int k = 0; k < E / 4; ++k) {
+    for (int k = 0; k < kRounds; ++k) {
       const int i = i0 + at(k, 0);
       if (i + 4 <= V) {
         __builtin_memcpy(&x[4 * k], row + i, 16);   // (rows start on any multiple of 4 bytes)
@@ -211,70 +239,96 @@ struct Chunk {
     for (int e = 0; e < E; ++e) m = max(m, order(x[e]));
     return m;
   }
-  // The entry at which the running sum of what stays passes target, given the sum
-  // before these; -1: not among them. sum: of these. red: NT / 64 + 2 words.
-  __device__ int pick(const Keep& keep, uint64_t before, uint64_t target, bool whole, float u, uint64_t* part, uint64_t* red) {
-    constexpr int K = E / 4;
-    // sums of the K rounds of 4 NT entries
-    for (int k = threadIdx.x; k < K; k += NT) part[k] = 0;
-    __syncthreads();
+  // the first index of value v
+  __device__ int first(float v, uint64_t* red) const {
+    uint32_t i = 0xffffffffu;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      uint64_t s = 0;
+    for (int e = 0; e < E; ++e)
+      if (x[e] == v) i = min(i, (uint32_t)at(e / 4, e % 4));
+    return (int)~group_max<NT>(~i, red);
+  }
+  // The first entry at which the running sum of what stays, from `before` on,
+  // passes target (whole: passes target times the sum of these); where rounding
+  // leaves none, the last that stays. part: kRounds * NT / 64 words, red: NT / 64 + 1.
+  __device__ int pick(const Keep& keep, double before, double target, bool whole, double* part, uint64_t* red) const {
+    constexpr int W = NT / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double w[E];
+    uint32_t any = 0;   // 1 + the last entry with a weight
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s += keep(x[4 * k + j]);
-      s = wave_sum_u64(s);
-      if ((threadIdx.x & 63) == 0 && s) add_u64(&part[k], s);
-    }
-    __syncthreads();
-    if (whole) {   // the row is these entries: the draw goes by their sum
-      uint64_t total = 0;
-      for (int k = 0; k < K; ++k) total += part[k];
-      target = draw_target(u, total);
-    }
-    int kf = -1;
-    uint64_t at_k = before;
-    for (int k = 0; k < K; ++k) {
-      if (kf < 0 && target < at_k + part[k]) kf = k;
-      if (kf < 0) at_k += part[k];
-    }
-    if (kf < 0) return -1;   // (uniform)
-    uint64_t w[4] = {}, s = 0;
+    for (int k = 0; k < kRounds; ++k) {
+      double s = 0.0;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (k == kf) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s += w[j] = keep(x[4 * k + j]);
+      for (int j = 0; j < 4; ++j) {
+        w[4 * k + j] = keep(x[4 * k + j]);
+        s += w[4 * k + j];
+        if (w[4 * k + j] > 0.0) any = at(k, j) + 1;
       }
-    uint64_t all;
-    uint64_t c = at_k + sum_before<NT>(s, red, all);
-    int* found = reinterpret_cast<int*>(red + NT / 64);
-    if (c <= target && target < c + s) {   // one thread
-      int j = 0;
-      while (c + w[j] <= target) c += w[j++];
-      *found = at(kf, j);
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
+      if (lane == 0) part[W * k + wave] = s;
+    }
+    any = group_max<NT>(any, red);   // (and a barrier for part)
+    if (whole) {
+      double total = 0.0;
+      for (int p = 0; p < kRounds * W; ++p) total += part[p];
+      target *= total;
+    }
+    int* found = reinterpret_cast<int*>(red + W);
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    // the wave and round that the draw falls into look closer
+    double c = before;
+    int p = 0;
+    while (p < kRounds * W && !(target < c + part[p])) c += part[p++];
+    if (p < kRounds * W && wave == p % W) {
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k)
+        if (k == p / W) {
+          const double s = (w[4 * k] + w[4 * k + 1]) + (w[4 * k + 2] + w[4 * k + 3]);
+          double incl = s;
+#pragma unroll
+          for (int off = 1; off < kWave; off <<= 1) {
+            const double o = __shfl_up(incl, off, kWave);
+            if (lane >= off) incl += o;
+          }
+          double at0 = c + (incl - s);
+          int mine = -1, held = -1;   // the first to pass, the last that stays
+#pragma unroll
+          for (int j = 3; j >= 0; --j) {
+            double upto = at0;
+#pragma unroll
+            for (int i = 0; i <= j; ++i) upto += w[4 * k + i];
+            if (w[4 * k + j] > 0.0 && target < upto) mine = at(k, j);
+            if (w[4 * k + j] > 0.0 && held < 0) held = at(k, j);
+          }
+          const uint64_t hit = __ballot(mine >= 0), some = __ballot(held >= 0);
+          if (hit ? lane == __ffsll((unsigned long long)hit) - 1 : some && lane == 63 - __clzll((long long)some))
+            *found = hit ? mine : held;
+        }
     }
     __syncthreads();
-    return *found;
+    return *found >= 0 ? *found : (int)any - 1;
   }
 };
 
 // ---- the thresholds --------------------------------------------------------------
 // Where the highest of the thresholds lies, from the bins' entries and weights.
 struct Edge {
-  int bin;             // of the threshold (the one below all kBins: everything stays)
+  int r;               // of bin top - r (kBins: everything stays)
   uint64_t need_k;     // entries of that bin that stay by top-k (0: no limit there)
-  uint64_t need_p;     // weight of that bin, as bin_weight, at which top-p cuts (0: none there)
+  uint64_t need_p;     // weight of that bin, as Scale::weight, at which top-p cuts (0: none there)
+  __device__ __forceinline__ bool inside() const { return need_k || need_p; }
 };
 struct Bins {
-  uint64_t weight[kBins];   // [top - bin]
+  uint64_t weight[kBins];   // [r]
   uint32_t count[kBins];
 };
 
-// by the first wave, from bins in LDS; lane l has bins l and 64 + l
-__device__ __forceinline__ Edge find_edge(const SampleRowsArgs& a, const Bins& h, int top, float mx, double per) {
+// by one wave, from bins in LDS; lane l has bins l and 64 + l
+__device__ __forceinline__ Edge find_edge(const SampleRowsArgs& a, const Bins& h, const Keep& keep) {
   const int lane = threadIdx.x & 63;
-  int kb = kBins, pb = kBins;
+  int kb = kBins, pb = kBins, mb = kBins;
   uint64_t need_k = 0, need_p = 0;
   if (a.top_k) {
     uint64_t base = 0;
@@ -297,11 +351,10 @@ __device__ __forceinline__ Edge find_edge(const SampleRowsArgs& a, const Bins& h
     }
   }
   if (a.top_p < 1.0) {
-    // in units of the top bin's middle
     double m[2], incl[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      m[half] = (double)h.weight[64 * half + lane] * exp(-0.25 * (64 * half + lane));
+      m[half] = (double)h.weight[64 * half + lane] * keep.fall[64 * half + lane];
       incl[half] = m[half];
 #pragma unroll
       for (int off = 1; off < kWave; off <<= 1) {
@@ -311,91 +364,97 @@ __device__ __forceinline__ Edge find_edge(const SampleRowsArgs& a, const Bins& h
     }
     incl[1] += __shfl(incl[0], 63, kWave);
     const double goal = a.top_p * __shfl(incl[1], 63, kWave);
-    for (int half = 0; half < 2 && pb == kBins; ++half) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
       const uint64_t hit = __ballot(incl[half] >= goal);
-      if (hit) {
+      if (hit && pb == kBins) {
         const int l = __ffsll((unsigned long long)hit) - 1;
         pb = 64 * half + l;
-        const double above = __shfl(incl[half] - m[half], l, kWave);
-        const uint64_t whole = __shfl((unsigned long long)h.weight[64 * half + lane], l, kWave);
-        need_p = min((uint64_t)fmax(ceil((goal - above) * exp(0.25 * pb)), 1.0), whole);
+        const uint64_t in = __shfl((unsigned long long)h.weight[pb], 0, kWave);
+        const double need = (goal - __shfl(incl[half] - m[half], l, kWave)) / keep.fall[pb];
+        need_p = min((uint64_t)fmax(ceil(need), 1.0), in);
       }
     }
   }
-  int mb = kBins;
-  if (a.min_gap > -INFINITY) {
-    const double b = floor(((double)mx + a.min_gap) * per);
-    mb = b <= (double)top - kBins ? kBins : b >= (double)top ? 0 : top - (int)b;
+  if (keep.min_gap > -INFINITY) {
+    const float r = keep.top - keep.scale.bin((float)((double)keep.mx + keep.min_gap));
+    mb = r < kBins ? (int)fmaxf(r, 0.f) : kBins;
   }
   const int r = min(min(kb, pb), mb);
-  Edge e;
-  e.bin = top - r;
-  e.need_k = kb == r ? need_k : 0;
-  e.need_p = pb == r ? need_p : 0;
-  return e;
+  return {r, kb == r ? need_k : 0, pb == r ? need_p : 0};
 }
 
 // The least key that stays, among the n entries of the threshold's bin (v: their
-// logits, in LDS): a thread of the workgroup for each, or selection by bits.
+// logits, in LDS): each compared with all, by 8 threads, or selection by bits.
+// digits: kDigits words.
 template <int NT>
-__device__ uint32_t least_of(const Edge& e, const float* v, int n, double per, uint64_t* hist, uint64_t* red, uint32_t* least) {
+__device__ uint32_t least_of(const Edge& e, const Keep& keep, const float* v, int n, uint64_t* digits, uint64_t* red,
+                             uint32_t* least) {
+  const float bin = keep.top - (float)e.r;
+  const int tid = threadIdx.x;
   if (n <= kPairs) {
+    static_assert(kPairs <= kDigits && kPairs <= NT, "a weight per entry");
+    if (tid < n) digits[tid] = e.need_p ? keep.scale.weight(v[tid], bin) : 0;
+    if (tid == 0) *least = 0;
     __syncthreads();
-    if (threadIdx.x == 0) *least = 0;
-    __syncthreads();
-    if ((int)threadIdx.x < n) {
-      const float x = v[threadIdx.x];
-      uint64_t ge = 0, gt = 0, wge = 0, wgt = 0;   // entries and weights at or above x, and above
-      for (int j = 0; j < n; ++j) {
+    for (int i = tid / 8; i < n; i += NT / 8) {
+      const float x = v[i];
+      uint32_t ge = 0, gt = 0;        // entries at or above x, and above
+      uint64_t wge = 0, wgt = 0;      // and their weights
+      for (int j = tid % 8; j < n; j += 8) {
         const float y = v[j];
-        const uint64_t w = e.need_p && y >= x ? bin_weight(y, per, e.bin) : 0;
+        const uint64_t w = digits[j];
         ge += y >= x;
         gt += y > x;
-        wge += w;
+        wge += y >= x ? w : 0;
         wgt += y > x ? w : 0;
       }
-      uint32_t k = 0;
-      if (e.need_k && gt < e.need_k && ge >= e.need_k) k = order(x);
-      if (e.need_p && wgt < e.need_p && wge >= e.need_p) k = max(k, order(x));
-      if (k) atomicMax(least, k);
+      uint64_t c = (uint64_t)gt << 32 | ge;
+#pragma unroll
+      for (int off = 1; off < 8; off <<= 1) {
+        c += __shfl_xor((unsigned long long)c, off, kWave);
+        wge += __shfl_xor((unsigned long long)wge, off, kWave);
+        wgt += __shfl_xor((unsigned long long)wgt, off, kWave);
+      }
+      const bool by_k = e.need_k && (c >> 32) < e.need_k && (uint32_t)c >= e.need_k;
+      const bool by_p = e.need_p && wgt < e.need_p && wge >= e.need_p;
+      if (tid % 8 == 0 && (by_k || by_p)) atomicMax(least, order(x));
     }
     __syncthreads();
     return *least;
   }
+  auto key = [&](int i) { return order(v[i]); };
   uint32_t k = 0;
-  if (e.need_k) k = key_reaching<NT>(n, e.need_k, hist, red, [&](int i) { return order(v[i]); }, [](int) { return 1ull; });
-  if (e.need_p)
-    k = max(k, key_reaching<NT>(n, e.need_p, hist, red, [&](int i) { return order(v[i]); },
-                                [&](int i) { return bin_weight(v[i], per, e.bin); }));
+  if (e.need_k) k = key_reaching<NT>(n, e.need_k, digits, red, key, [](int) { return 1ull; });
+  if (e.need_p) k = max(k, key_reaching<NT>(n, e.need_p, digits, red, key, [&](int i) { return keep.scale.weight(v[i], bin); }));
   return k;
 }
 
-// A whole row by one workgroup without bins.
+// A whole row by one workgroup without bins, with weights of up to 2^44.
 template <int NT>
 __device__ int slow(const SampleRowsArgs& a, const float* x, float mx, float u, uint64_t* hist, uint64_t* red) {
   const int V = a.V, tid = threadIdx.x;
-  Keep keep = {0, mx, a.temperature, -INFINITY};
   auto key = [&](int i) { return order(x[i]); };
+  auto weight = [&](int i) { return (uint64_t)(exp(gap(x[i], mx) / a.temperature) * kUnit + 0.5); };
   uint32_t least = 0;
   if (a.top_k) least = key_reaching<NT>(V, (uint64_t)a.top_k, hist, red, key, [](int) { return 1ull; });
   if (a.top_p < 1.0) {
     uint64_t s = 0;
-    for (int i = tid; i < V; i += NT) s += keep(x[i]);
+    for (int i = tid; i < V; i += NT) s += weight(i);
     const double goal = ceil(a.top_p * (double)group_sum<NT>(s, red));
-    least = max(least, key_reaching<NT>(V, (uint64_t)fmax(goal, 1.0), hist, red, key, [&](int i) { return keep(x[i]); }));
+    least = max(least, key_reaching<NT>(V, (uint64_t)fmax(goal, 1.0), hist, red, key, weight));
   }
-  keep.least = least;
-  keep.min_gap = a.min_gap;
+  auto kept = [&](int i) { return key(i) >= least && gap(x[i], mx) >= a.min_gap ? weight(i) : 0; };
   // contiguous pieces: the thread in whose piece the running sum passes the draw
   const int C = (V + NT - 1) / NT, i0 = min(tid * C, V), i1 = min(i0 + C, V);
   uint64_t s = 0, total;
-  for (int i = i0; i < i1; ++i) s += keep(x[i]);
+  for (int i = i0; i < i1; ++i) s += kept(i);
   uint64_t c = sum_before<NT>(s, red, total);
-  const uint64_t target = draw_target(u, total);
+  const uint64_t target = min((uint64_t)(fraction(u) * (double)total), total - 1);   // (the maximum stays: total > 0)
   int* found = reinterpret_cast<int*>(red + NT / 64);
   if (c <= target && target < c + s) {   // one thread
     int i = i0;
-    for (c += keep(x[i]); c <= target; c += keep(x[i])) ++i;
+    for (c += kept(i); c <= target; c += kept(i)) ++i;
     *found = i;
   }
   __syncthreads();
@@ -413,12 +472,12 @@ struct Histogram {
       (&count[0][0])[i] = 0;
     }
   }
-  __device__ __forceinline__ void add(float x, int top, double per, bool weights) {
-    const int b = bin_of(x, per), r = top - b;
-    if (r >= kBins) return;
+  __device__ __forceinline__ void add(float x, float top, const Scale& s, bool counts, bool weights) {
+    const float b = s.bin(x), r = top - b;
+    if (!(r < kBins)) return;
     const int c = threadIdx.x % kCopies;
-    atomicAdd(&count[r][c], 1u);
-    if (weights) add_u64(&weight[r][c], bin_weight(x, per, b));
+    if (counts) atomicAdd(&count[(int)r][c], 1u);
+    if (weights) add_u64(&weight[(int)r][c], s.weight(x, b));
   }
   __device__ __forceinline__ void sum(int r, uint64_t& w, uint32_t& n) const {
     w = 0;
@@ -431,85 +490,75 @@ struct Histogram {
   }
 };
 
+__device__ __forceinline__ Scale scale_of(const SampleRowsArgs& a) { return {(float)(4.0 / a.temperature), 1.0 / a.temperature}; }
+__device__ __forceinline__ bool filtered(const SampleRowsArgs& a) { return a.top_k || a.top_p < 1.0; }
+// neighbouring bins are told apart around this one
+__device__ __forceinline__ bool is_near(float top) { return top > -kFar && top < kFar; }
+
 // ---- one workgroup per row ---------------------------------------------------------
-template <int E>
 __global__ void __launch_bounds__(kOneThreads) k_one(const SampleRowsArgs a) {
   constexpr int NT = kOneThreads;
+  using Row = Chunk<NT, kOne / NT>;
   __shared__ union {
     Histogram<NT> h;
-    float v[kList];
+    float v[kOne];
   } sh;
   __shared__ Bins bins;
-  __shared__ uint64_t red[NT / 64 + 2], part[E / 4], digits[256];
+  __shared__ double fall[kBins], part[Row::kRounds * NT / 64];
+  __shared__ uint64_t red[NT / 64 + 2], digits[kDigits];
   __shared__ uint32_t least;
   __shared__ int n;
   __shared__ Edge edge;
   const int tid = threadIdx.x, row = blockIdx.x;
   const float* x = a.logits + (size_t)row * a.ld;
-  Chunk<NT, E> c;
+  Row c;
   c.load(x, 0, a.V);
-  const uint32_t mk = group_max<NT>(c.top(), red);
-  const float mx = from_order(mk);
-  if (mx == -INFINITY) {   // nothing to choose from
-    if (tid == 0) a.out[row] = -1;
-    return;
-  }
-  if (!(a.temperature > 0.0)) {
-    uint32_t first = 0xffffffffu;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (c.x[e] == mx) first = min(first, (uint32_t)c.at(e / 4, e % 4));
-    first = ~group_max<NT>(~first, red);
-    if (tid == 0) a.out[row] = (int)first;
+  if (tid < kBins) fall[tid] = exp(-0.25 * tid);
+  if (filtered(a)) sh.h.clear();
+  if (tid == 0) n = 0;
+  const float mx = from_order(group_max<NT>(c.top(), red));
+  if (mx == -INFINITY || !(a.temperature > 0.0)) {   // nothing to choose from, or the first maximum
+    const int i = mx == -INFINITY ? -1 : c.first(mx, red);
+    if (tid == 0) a.out[row] = i;
     return;
   }
   const float u = a.u[row];
-  Keep keep = {0, mx, a.temperature, a.min_gap};
-  if (a.top_k || a.top_p < 1.0) {
-    const double per = 4.0 / a.temperature;
-    const int top = bin_of(mx, per);
-    sh.h.clear();
-    if (tid == 0) n = 0;
-    __syncthreads();
+  const Scale scale = scale_of(a);
+  Keep keep = {scale, fall, scale.bin(mx), mx, a.min_gap, 0};
+  if (!is_near(keep.top)) {
+    const int i = slow<NT>(a, x, mx, u, digits, red);
+    if (tid == 0) a.out[row] = i;
+    return;
+  }
+  if (filtered(a)) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) sh.h.add(c.x[e], top, per, a.top_p < 1.0);
+    for (int e = 0; e < kOne / NT; ++e) sh.h.add(c.x[e], keep.top, scale, a.top_k, a.top_p < 1.0);
     __syncthreads();
     if (tid < kBins) sh.h.sum(tid, bins.weight[tid], bins.count[tid]);
     __syncthreads();
     if (tid < kWave) {
-      const Edge e = find_edge(a, bins, top, mx, per);
+      const Edge e = find_edge(a, bins, keep);
       if (tid == 0) edge = e;
     }
     __syncthreads();
     const Edge e = edge;
-    const bool far = top <= -kFar || top >= kFar;
-    if (e.need_k || e.need_p || far) {
-      if (far || bins.count[top - e.bin] > (uint32_t)kList) {
-        const int i = slow<NT>(a, x, mx, u, digits, red);
-        if (tid == 0) a.out[row] = i;
-        return;
-      }
+    if (e.inside()) {   // (else min-p alone cuts there, and the entries are asked one by one)
 #pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (bin_of(c.x[k], per) == e.bin) sh.v[atomicAdd(&n, 1)] = c.x[k];
+      for (int k = 0; k < kOne / NT; ++k)
+        if (keep.top - scale.bin(c.x[k]) == (float)e.r) sh.v[atomicAdd(&n, 1)] = c.x[k];
       __syncthreads();
-      keep.least = least_of<NT>(e, sh.v, n, per, digits, red, &least);
-    }   // (else min-p alone cuts there, and the entries are asked one by one)
+      keep.least = least_of<NT>(e, keep, sh.v, n, digits, red, &least);
+    }
   }
-  __syncthreads();
-  const int i = c.pick(keep, 0, 0, true, u, part, red);
+  const int i = c.pick(keep, 0.0, fraction(u), true, part, red);
   if (tid == 0) a.out[row] = i;
 }
-
 // ---- many workgroups per row -------------------------------------------------------
 // A row's part of the workspace
 struct RowWork {
   Bins* bins;          // [tiles], each from its own maximum's bin down
   uint32_t* top;       // [tiles] the maximum's key
   int* first;          // [tiles] temperature 0: its first index
-  uint64_t* kept;      // [tiles] weights that stay for certain
-  uint64_t* list;      // [kList] the threshold's bin: index << 32 | x
-  uint32_t* count;     // [0] entries of that list, [1] workgroups done
 };
 __host__ __device__ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 __host__ __device__ inline RowWork row_work(void* work, int row, int tiles, size_t* bytes) {
@@ -519,75 +568,71 @@ __host__ __device__ inline RowWork row_work(void* work, int row, int tiles, size
     o += up256(n);
     return at;
   };
-  const size_t b = take(sizeof(Bins) * tiles), t = take(sizeof(uint32_t) * tiles), f = take(sizeof(int) * tiles),
-               k = take(sizeof(uint64_t) * tiles), l = take(sizeof(uint64_t) * kList), c = take(2 * sizeof(uint32_t));
+  const size_t b = take(sizeof(Bins) * tiles), t = take(sizeof(uint32_t) * tiles), f = take(sizeof(int) * tiles);
   uint8_t* p = static_cast<uint8_t*>(work) + (size_t)row * o;
   if (bytes) *bytes = o;
-  return {reinterpret_cast<Bins*>(p + b),     reinterpret_cast<uint32_t*>(p + t), reinterpret_cast<int*>(p + f),
-          reinterpret_cast<uint64_t*>(p + k), reinterpret_cast<uint64_t*>(p + l), reinterpret_cast<uint32_t*>(p + c)};
+  return {reinterpret_cast<Bins*>(p + b), reinterpret_cast<uint32_t*>(p + t), reinterpret_cast<int*>(p + f)};
 }
-__host__ __device__ inline bool by_bins(const SampleRowsArgs& a) { return a.temperature > 0.0 && (a.top_k || a.top_p < 1.0); }
 
 // 1. a tile's maximum and bins. Grid: tiles x rows.
+template <int E>
 __global__ void __launch_bounds__(kTileThreads) k_tiles(const SampleRowsArgs a) {
   constexpr int NT = kTileThreads;
   __shared__ Histogram<NT> h;
   __shared__ uint64_t red[NT / 64 + 2];
   const int tid = threadIdx.x, tile = blockIdx.x, row = blockIdx.y;
   const RowWork w = row_work(a.work, row, gridDim.x, nullptr);
-  Chunk<NT, kTileEach> c;
-  c.load(a.logits + (size_t)row * a.ld, tile * kTile, a.V);
-  if (by_bins(a)) h.clear();
+  Chunk<NT, E> c;
+  c.load(a.logits + (size_t)row * a.ld, tile * NT * E, a.V);
+  h.clear();
   const uint32_t mk = group_max<NT>(c.top(), red);
-  if (tid == 0) {
-    w.top[tile] = mk;
-    if (tile == 0) w.count[0] = w.count[1] = 0;
-  }
+  if (tid == 0) w.top[tile] = mk;
   const float mx = from_order(mk);
+  if (mx == -INFINITY) return;
   if (!(a.temperature > 0.0)) {
-    uint32_t first = 0xffffffffu;
-#pragma unroll
-    for (int e = 0; e < kTileEach; ++e)
-      if (c.x[e] == mx) first = min(first, (uint32_t)c.at(e / 4, e % 4));
-    first = ~group_max<NT>(~first, red);
-    if (tid == 0) w.first[tile] = tile * kTile + (int)first;
+    const int i = c.first(mx, red);
+    if (tid == 0) w.first[tile] = tile * NT * E + i;
+    return;
   }
-  if (!by_bins(a) || mx == -INFINITY) return;
-  const double per = 4.0 / a.temperature;
-  const int top = bin_of(mx, per);
+  const Scale scale = scale_of(a);
+  const float top = scale.bin(mx);
 #pragma unroll
-  for (int e = 0; e < kTileEach; ++e) h.add(c.x[e], top, per, a.top_p < 1.0);
+  for (int e = 0; e < E; ++e) h.add(c.x[e], top, scale, a.top_k, true);
   __syncthreads();
   if (tid < kBins) h.sum(tid, w.bins[tile].weight[tid], w.bins[tile].count[tid]);
 }
 
-// 2. what stays of each tile; the row's last workgroup draws. Grid: tiles x rows.
-__global__ void __launch_bounds__(kTileThreads) k_draw(const SampleRowsArgs a) {
-  constexpr int NT = kTileThreads, kGroups = NT / kBins;
-  __shared__ union {
-    Bins part[kGroups];
-    struct {
-      float v[kList];
-      int at[kList];
-    } l;
-  } sh;
+// 2. threshold and token. Grid: rows.
+template <int E>
+__global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, int tiles) {
+  constexpr int NT = kRowThreads, kTile = kTileThreads * E, kWaves = NT / 64;
+  constexpr int kMost = (kMaxTiles * 8 / E + kWaves - 1) / kWaves;   // tiles of a wave
+  using Tile = Chunk<NT, kTile / NT>;
+  __shared__ float v[kList];
+  __shared__ int at[kList];
   __shared__ Bins bins;
-  __shared__ uint64_t red[NT / 64 + 2], part[kTileEach / 4], digits[256], kept[kMaxTiles];
-  __shared__ uint32_t tops[kMaxTiles], least, base;
+  __shared__ double fall[kBins], kept[kMaxTiles], part[Tile::kRounds * kWaves];
+  __shared__ uint64_t red[kWaves + 2], digits[kDigits], edge_kept[kMaxTiles];
+  __shared__ uint32_t tops[kMaxTiles], least;
+  __shared__ int n;
+  __shared__ bool there[kMaxTiles];   // the tile has entries in the threshold's bin
   __shared__ Edge edge;
-  __shared__ bool last;
-  const int tid = threadIdx.x, tile = blockIdx.x, tiles = gridDim.x, row = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
   const RowWork w = row_work(a.work, row, tiles, nullptr);
   const float* x = a.logits + (size_t)row * a.ld;
-  Chunk<NT, kTileEach> c;
-  c.load(x, tile * kTile, a.V);
-  if (tid < tiles) tops[tid] = w.top[tid];
+  for (int t = tid; t < tiles; t += NT) tops[t] = w.top[t];
+  if (tid < kBins) {
+    fall[tid] = exp(-0.25 * tid);
+    bins.weight[tid] = 0;
+    bins.count[tid] = 0;
+  }
+  if (tid == 0) n = 0;
   __syncthreads();
   uint32_t mk = 0;
   for (int t = 0; t < tiles; ++t) mk = max(mk, tops[t]);
   const float mx = from_order(mk);
   if (mx == -INFINITY || !(a.temperature > 0.0)) {   // nothing to choose from, or the first maximum
-    if (tile == 0 && tid == 0) {
+    if (tid == 0) {
       int t = 0;
       while (tops[t] != mk) ++t;
       a.out[row] = mx == -INFINITY ? -1 : w.first[t];
@@ -595,134 +640,159 @@ __global__ void __launch_bounds__(kTileThreads) k_draw(const SampleRowsArgs a) {
     return;
   }
   const float u = a.u[row];
-  const double per = 4.0 / a.temperature;
-  const int top = bin_of(mx, per);
-  Keep keep = {0, mx, a.temperature, a.min_gap};
-  Edge e = {top - kBins, 0, 0};
-  if (by_bins(a)) {
-    const int r = tid % kBins, g = tid / kBins;
-    uint64_t weight = 0;
-    uint32_t count = 0;
-    for (int t = g; t < tiles; t += kGroups) {
-      const float m = from_order(tops[t]);
-      if (m == -INFINITY) continue;
-      const int at = r - (top - bin_of(m, per));
-      if (at < 0) continue;
-      weight += w.bins[t].weight[at];
-      count += w.bins[t].count[at];
-    }
-    sh.part[g].weight[r] = weight;
-    sh.part[g].count[r] = count;
-    __syncthreads();
-    if (tid < kBins) {
-      uint64_t s = 0;
-      uint32_t n = 0;
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        s += sh.part[k].weight[tid];
-        n += sh.part[k].count[tid];
-      }
-      bins.weight[tid] = s;
-      bins.count[tid] = n;
-    }
-    __syncthreads();
-    if (tid < kWave) {
-      const Edge f = find_edge(a, bins, top, mx, per);
-      if (tid == 0) edge = f;
-    }
-    __syncthreads();
-    e = edge;
-  }
-  const bool far = by_bins(a) && (top <= -kFar || top >= kFar);
-  const bool inside = e.need_k || e.need_p;   // the threshold is found among the bin's entries
-  uint64_t s = 0;
-  int mine = 0;
-  if (!far) {
-#pragma unroll
-    for (int k = 0; k < kTileEach; ++k) {
-      const int b = inside ? bin_of(c.x[k], per) : 0;
-      if (!inside || b > e.bin) s += keep(c.x[k]);
-      else if (b == e.bin) ++mine;
-    }
-  }
-  s = group_sum<NT>(s, red);
-  uint64_t all;
-  int at = (int)sum_before<NT>((uint64_t)mine, red, all);
-  if (tid == 0) {
-    cst64(&w.kept[tile], s);
-    base = all ? __hip_atomic_fetch_add(&w.count[0], (uint32_t)all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
-  }
-  __syncthreads();
-  if (mine) {
-    at += (int)base;
-#pragma unroll
-    for (int k = 0; k < kTileEach; ++k)
-      if (bin_of(c.x[k], per) == e.bin) {
-        if (at < kList)
-          cst64(&w.list[at], (uint64_t)(uint32_t)(tile * kTile + c.at(k / 4, k % 4)) << 32 | __float_as_uint(c.x[k]));
-        ++at;
-      }
-  }
-  vm_drain();   // what this wave published
-  __syncthreads();
-  if (tid == 0)
-    last = __hip_atomic_fetch_add(&w.count[1], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)tiles - 1;
-  __syncthreads();
-  if (!last) return;
-
-  const uint32_t n = cld(&w.count[0]);
-  if (far || n > (uint32_t)kList) {
+  const Scale scale = scale_of(a);
+  Keep keep = {scale, fall, scale.bin(mx), mx, a.min_gap, 0};
+  if (!is_near(keep.top)) {
     const int i = slow<NT>(a, x, mx, u, digits, red);
     if (tid == 0) a.out[row] = i;
     return;
   }
-  if (tid < tiles) kept[tid] = cld64(&w.kept[tid]);
-  for (int i = tid; i < (int)n; i += NT) {
-    const uint64_t y = cld64(&w.list[i]);
-    sh.l.v[i] = __uint_as_float((uint32_t)y);
-    sh.l.at[i] = (int)(y >> 32);
+  // the tiles' bins, tile t in wave t % 16, bins lane and 64 + lane of the row's;
+  // a tile's own begin `shift` bins further down
+  uint64_t weight[kMost][2];
+  uint32_t count[kMost][2];
+#pragma unroll
+  for (int k = 0; k < kMost; ++k) {
+    const int t = wave + k * kWaves;
+    int shift = kBins;
+    if (t < tiles) {
+      const float m = from_order(tops[t]), d = keep.top - scale.bin(m);
+      if (m > -INFINITY && d < kBins) shift = (int)d;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = lane + 64 * h - shift;
+      weight[k][h] = r >= 0 ? w.bins[t].weight[r] : 0;
+      count[k][h] = r >= 0 ? w.bins[t].count[r] : 0;
+    }
+  }
+  if (filtered(a)) {
+#pragma unroll
+    for (int k = 0; k < kMost; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (weight[k][h]) add_u64(&bins.weight[lane + 64 * h], weight[k][h]);
+        if (count[k][h]) atomicAdd(&bins.count[lane + 64 * h], count[k][h]);
+      }
   }
   __syncthreads();
-  if (inside) {
-    keep.least = least_of<NT>(e, sh.l.v, (int)n, per, digits, red, &least);
-    for (int i = tid; i < (int)n; i += NT)
-      if (const uint64_t v = keep(sh.l.v[i])) add_u64(&kept[sh.l.at[i] / kTile], v);
+  if (tid < kWave) {
+    const Edge f = find_edge(a, bins, keep);
+    if (tid == 0) edge = f;
+  }
+  __syncthreads();
+  const Edge e = edge;
+  // a tile's weights above the threshold's bin
+#pragma unroll
+  for (int k = 0; k < kMost; ++k) {
+    const int t = wave + k * kWaves;
+    if (t >= tiles) break;
+    double s = 0.0;
+    bool some = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = lane + 64 * h;
+      if (r < e.r) s += (double)weight[k][h] * fall[r];
+      some = some || (r == e.r && weight[k][h] > 0);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
+    const bool any = __any(some);
+    if (lane == 0) {
+      kept[t] = s;
+      edge_kept[t] = 0;
+      there[t] = any;
+    }
+  }
+  __syncthreads();
+  if (e.r < kBins) {
+    // that bin's entries: into the list, or, where min-p alone cuts, those that pass
+    const float bin = keep.top - (float)e.r;
+    for (int i0 = 0; i0 < a.V; i0 += kRounds * 4 * NT) {
+      Chunk<NT, 4> c[kRounds];
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k) {
+        const int i = i0 + 4 * k * NT;
+        if (i < a.V && there[i / kTile]) c[k].load(x, i, a.V);
+      }
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k) {
+        const int i = i0 + 4 * k * NT;
+        if (i >= a.V || !there[i / kTile]) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (scale.bin(c[k].x[j]) != bin) continue;
+          if (!e.inside()) {
+            if (gap(c[k].x[j], mx) >= a.min_gap) add_u64(&edge_kept[i / kTile], scale.weight(c[k].x[j], bin));
+          } else if (const int p = atomicAdd(&n, 1); p < kList) {
+            v[p] = c[k].x[j];
+            at[p] = i + c[k].at(0, j);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (n > kList) {
+      const int i = slow<NT>(a, x, mx, u, digits, red);
+      if (tid == 0) a.out[row] = i;
+      return;
+    }
+    if (e.inside()) {
+      keep.least = least_of<NT>(e, keep, v, n, digits, red, &least);
+      for (int i = tid; i < n; i += NT)
+        if (keep(v[i]) > 0.0) add_u64(&edge_kept[at[i] / kTile], scale.weight(v[i], bin));
+      __syncthreads();
+    }
+    for (int t = tid; t < tiles; t += NT) kept[t] += (double)edge_kept[t] * fall[e.r];
     __syncthreads();
   }
-  uint64_t total = 0, before = 0;
-  for (int t = 0; t < tiles; ++t) total += kept[t];
-  const uint64_t target = draw_target(u, total);
+  double total = 0.0, before = 0.0;
+  int held = 0;   // the last tile with a weight
+  for (int t = 0; t < tiles; ++t) {
+    total += kept[t];
+    if (kept[t] > 0.0) held = t;
+  }
+  const double target = fraction(u) * total;
   int t = 0;
-  while (t < tiles - 1 && target >= before + kept[t]) before += kept[t++];
+  while (t < held && !(target < before + kept[t])) before += kept[t++];
+  Tile c;
   c.load(x, t * kTile, a.V);
-  const int i = c.pick(keep, before, target, false, u, part, red);
+  const int i = c.pick(keep, before, target, false, part, red);
   if (tid == 0) a.out[row] = t * kTile + i;
 }
 
+// entries a thread of the tiles has: 8 where that gives a workgroup for every two
+// compute units at most
+int entries_of(int rows, int V, int n_cu) {
+  return (int64_t)rows * ((V + 8 * kTileThreads - 1) / (8 * kTileThreads)) * 2 <= n_cu ? 8 : 16;
+}
+int tiles_of(int rows, int V, int n_cu) {
+  const int tile = entries_of(rows, V, n_cu) * kTileThreads;
+  return V <= kOne ? 0 : (V + tile - 1) / tile;
+}
+
 template <int E>
-hipError_t launch_one(const SampleRowsArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(k_one<E>, dim3(a.rows), dim3(kOneThreads), 0, s, a);
+hipError_t launch_tiles(const SampleRowsArgs& a, int tiles, hipStream_t s) {
+  const dim3 grid(tiles, a.rows), block(kTileThreads);
+  hipLaunchKernelGGL(k_tiles<E>, grid, block, 0, s, a);
+  hipLaunchKernelGGL(k_draw<E>, dim3(a.rows), dim3(kRowThreads), 0, s, a, tiles);
   return hipGetLastError();
 }
-int tiles_of(int V) { return V <= kOneMax ? 0 : (V + kTile - 1) / kTile; }
 
 }  // namespace
 
-size_t sample_rows_workspace(int rows, int V) {
+size_t sample_rows_workspace(int rows, int V, int n_cu) {
   size_t bytes = 0;
-  if (const int tiles = tiles_of(V)) row_work(nullptr, 0, tiles, &bytes);
+  if (const int tiles = tiles_of(rows, V, n_cu)) row_work(nullptr, 0, tiles, &bytes);
   return bytes * rows;
 }
 
 hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s) {
   if (a.rows < 1 || a.V < 1 || a.V > kSampleRowsMaxV) return hipErrorInvalidValue;
-  if (const int tiles = tiles_of(a.V)) {
-    const dim3 grid(tiles, a.rows), block(kTileThreads);
-    hipLaunchKernelGGL(k_tiles, grid, block, 0, s, a);
-    hipLaunchKernelGGL(k_draw, grid, block, 0, s, a);
-    return hipGetLastError();
-  }
-  return a.V <= 4 * kOneThreads ? launch_one<4>(a, s) : a.V <= 16 * kOneThreads ? launch_one<16>(a, s) : launch_one<kOneEach>(a, s);
+  if (const int tiles = tiles_of(a.rows, a.V, a.n_cu))
+    return entries_of(a.rows, a.V, a.n_cu) == 8 ? launch_tiles<8>(a, tiles, s) : launch_tiles<16>(a, tiles, s);
+  hipLaunchKernelGGL(k_one, dim3(a.rows), dim3(kOneThreads), 0, s, a);
+  return hipGetLastError();
 }
 
 }  // namespace ssk
