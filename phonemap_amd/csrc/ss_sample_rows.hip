@@ -28,6 +28,8 @@
 // entries in the threshold's bin, and draws within one tile. Weights are formed
 // once, for the histogram, and again for the threshold's bin and the last tile.
 
+#include <type_traits>
+
 #include "ss_device.h"
 #include "ss_kernels.h"
 
@@ -68,9 +70,9 @@ struct Scale {
   float per;
   double inv;
   __device__ __forceinline__ float bin(float x) const { return x == x ? floorf(x * per) : -INFINITY; }
-  // e^(x / T - the middle of bin b) in units of 2^-44, for |x / T - that| of 1/8 and a
-  // little: the ninth power's term is below 2e-13
-  __device__ __forceinline__ uint64_t weight(float x, float b) const {
+  // e^(x / T - the middle of bin b), for |x / T - that| of 1/8 and a little: the
+  // ninth power's term is below 2e-13
+  __device__ __forceinline__ double weight(float x, float b) const {
     const double r = fma((double)x, inv, -0.25 * ((double)b + 0.5));
     double p = 1.0 / 40320;
     p = fma(p, r, 1.0 / 5040);
@@ -80,33 +82,72 @@ struct Scale {
     p = fma(p, r, 1.0 / 6);
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    // p * 2^44 as a whole number: the low bits of its sum with 2^52 (p is below 2)
-    return (uint64_t)__double_as_longlong(fma(p, kUnit, 0x1p52)) & 0xfffffffffffffull;
+    return fma(p, r, 1.0);
+  }
+  // in units of 2^-44, as a whole number: the low bits of its sum with 2^52 (it is below 2)
+  __device__ __forceinline__ uint64_t units(float x, float b) const {
+    return (uint64_t)__double_as_longlong(fma(weight(x, b), kUnit, 0x1p52)) & 0xfffffffffffffull;
   }
 };
 
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+// ---- sums over waves and workgroups ----------------------------------------------
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp64(T v) {   // 0 where no lane gives one
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+}
+// sum of v (uint64_t or double) over the lanes up to this one
+template <class T>
+__device__ __forceinline__ T wave_upto(T v) {
+  v += dpp64<0x111, 0xf>(v);   // row_shr:1
+  v += dpp64<0x112, 0xf>(v);
+  v += dpp64<0x114, 0xf>(v);
+  v += dpp64<0x118, 0xf>(v);
+  v += dpp64<0x142, 0xa>(v);   // row_bcast:15 into rows 1 and 3
+  v += dpp64<0x143, 0xc>(v);   // row_bcast:31 into rows 2 and 3
   return v;
 }
-// over the workgroup of NT threads, in every thread; red: NT / 64 words
-template <int NT>
-__device__ uint64_t group_sum(uint64_t v, uint64_t* red) {
-  v = wave_sum_u64(v);
+template <class T>
+__device__ __forceinline__ T from_lane(T v, int lane) {   // lane: the same for the wave
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+}
+template <class T>
+__device__ __forceinline__ T wave_total(T v) {
+  return from_lane(wave_upto(v), 63);
+}
+// over the workgroup of NT threads, in every thread, the waves in order; red: NT / 64 words
+template <int NT, class T>
+__device__ T group_sum(T v, T* red) {
+  v = wave_total(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  uint64_t t = 0;
+  T t = 0;
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) t += red[w];
   return t;
 }
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  auto up = [&](auto ctrl, auto rows) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  up(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
+  up(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  up(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  up(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  up(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  up(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 template <int NT>
 __device__ uint32_t group_max(uint32_t v, uint64_t* red) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, off, kWave));
+  v = wave_max_u32(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -119,12 +160,7 @@ __device__ uint32_t group_max(uint32_t v, uint64_t* red) {
 template <int NT>
 __device__ uint64_t sum_before(uint64_t v, uint64_t* red, uint64_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t incl = v;
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const uint64_t o = __shfl_up(incl, off, kWave);
-    if (lane >= off) incl += o;
-  }
+  const uint64_t incl = wave_upto(v);
   __syncthreads();
   if (lane == 63) red[wave] = incl;
   __syncthreads();
@@ -137,19 +173,6 @@ __device__ uint64_t sum_before(uint64_t v, uint64_t* red, uint64_t& all) {
   }
   return before;
 }
-// the same of doubles, added in the order of the lanes and waves; red: NT / 64 words
-template <int NT>
-__device__ double group_sum(double v, double* red) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double t = 0.0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) t += red[w];
-  return t;
-}
 __device__ __forceinline__ void add_u64(uint64_t* p, uint64_t v) {
   atomicAdd(reinterpret_cast<unsigned long long*>(p), (unsigned long long)v);
 }
@@ -157,7 +180,7 @@ __device__ __forceinline__ void add_u64(uint64_t* p, uint64_t v) {
 // Selection by the bits of the keys, kDigit at a time: the largest key at which
 // the sum of val(i) over the entries i < n with that key or a greater one reaches
 // target, 0 when all together do not. hist: 2^kDigit words, red: NT / 64 + 2.
-constexpr int kDigit = 9, kDigits = 1 << kDigit;
+constexpr int kDigit = 10, kDigits = 1 << kDigit;
 template <int NT, class Key, class Val>
 __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_t* red, Key key, Val val) {
   static_assert(NT >= kDigits, "a digit per thread");
@@ -200,17 +223,29 @@ __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_
   return prefix;
 }
 
+// e^(-r / 4), r < kBins, as a product of powers
+__device__ __forceinline__ double fall_of(int r) {
+  constexpr double kPower[7] = {0.77880078307140486825, 0.60653065971263342360, 0.36787944117144232160, 0.13533528323661269189,
+                                0.01831563888873418029, 0.00033546262790251183882, 1.1253517471925911451e-7};   // e^(-2^i / 4)
+  double f = 1.0;
+#pragma unroll
+  for (int i = 0; i < 7; ++i) f *= r >> i & 1 ? kPower[i] : 1.0;
+  return f;
+}
+
 // What stays, and with which weight, in units of the middle of the maximum's bin.
 struct Keep {
   Scale scale;
-  const double* fall;   // e^(-r / 4) of bin top - r
-  float top, mx;
+  const double* fall;   // fall_of(r), r < kBins
+  float top, mx;        // the maximum's bin and the maximum
   double min_gap;
-  uint32_t least;       // the least key
+  float least;          // the least that stays by top-k and top-p
+  __device__ __forceinline__ bool stays(float x) const {   // (not a NaN; entries of 0 weight aside)
+    return x >= least && (min_gap == -INFINITY || gap(x, mx) >= min_gap);
+  }
   __device__ __forceinline__ double operator()(float x) const {
     const float b = scale.bin(x), r = top - b;
-    if (!(r < kBins) || order(x) < least || !(gap(x, mx) >= min_gap)) return 0.0;
-    return (double)scale.weight(x, b) * fall[(int)r];
+    return r < kBins && stays(x) ? scale.weight(x, b) * fall[(int)r] : 0.0;
   }
 };
 
@@ -264,9 +299,8 @@ struct Chunk {
         s += w[4 * k + j];
         if (w[4 * k + j] > 0.0) any = at(k, j) + 1;
       }
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
-      if (lane == 0) part[W * k + wave] = s;
+      s = wave_upto(s);
+      if (lane == 63) part[W * k + wave] = s;
     }
     any = group_max<NT>(any, red);   // (and a barrier for part)
     if (whole) {
@@ -286,13 +320,7 @@ struct Chunk {
       for (int k = 0; k < kRounds; ++k)
         if (k == p / W) {
           const double s = (w[4 * k] + w[4 * k + 1]) + (w[4 * k + 2] + w[4 * k + 3]);
-          double incl = s;
-#pragma unroll
-          for (int off = 1; off < kWave; off <<= 1) {
-            const double o = __shfl_up(incl, off, kWave);
-            if (lane >= off) incl += o;
-          }
-          double at0 = c + (incl - s);
+          const double at0 = c + (wave_upto(s) - s);
           int mine = -1, held = -1;   // the first to pass, the last that stays
 #pragma unroll
           for (int j = 3; j >= 0; --j) {
@@ -332,22 +360,16 @@ __device__ __forceinline__ Edge find_edge(const SampleRowsArgs& a, const Bins& h
   uint64_t need_k = 0, need_p = 0;
   if (a.top_k) {
     uint64_t base = 0;
-    for (int half = 0; half < 2 && kb == kBins; ++half) {
-      const uint64_t c = h.count[64 * half + lane];
-      uint64_t incl = c;
 #pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) {
-        const uint64_t o = __shfl_up(incl, off, kWave);
-        if (lane >= off) incl += o;
-      }
-      incl += base;
+    for (int half = 0; half < 2; ++half) {
+      const uint64_t c = h.count[64 * half + lane], incl = base + wave_upto(c);
       const uint64_t hit = __ballot(incl >= (uint64_t)a.top_k);
-      if (hit) {
+      if (hit && kb == kBins) {
         const int l = __ffsll((unsigned long long)hit) - 1;
         kb = 64 * half + l;
-        need_k = a.top_k - __shfl(incl - c, l, kWave);
+        need_k = a.top_k - from_lane(incl - c, l);
       }
-      base = __shfl(incl, 63, kWave);
+      base = from_lane(incl, 63);
     }
   }
   if (a.top_p < 1.0) {
@@ -355,24 +377,17 @@ __device__ __forceinline__ Edge find_edge(const SampleRowsArgs& a, const Bins& h
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       m[half] = (double)h.weight[64 * half + lane] * keep.fall[64 * half + lane];
-      incl[half] = m[half];
-#pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) {
-        const double o = __shfl_up(incl[half], off, kWave);
-        if (lane >= off) incl[half] += o;
-      }
+      incl[half] = wave_upto(m[half]) + (half ? from_lane(incl[0], 63) : 0.0);
     }
-    incl[1] += __shfl(incl[0], 63, kWave);
-    const double goal = a.top_p * __shfl(incl[1], 63, kWave);
+    const double goal = a.top_p * from_lane(incl[1], 63);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const uint64_t hit = __ballot(incl[half] >= goal);
       if (hit && pb == kBins) {
         const int l = __ffsll((unsigned long long)hit) - 1;
         pb = 64 * half + l;
-        const uint64_t in = __shfl((unsigned long long)h.weight[pb], 0, kWave);
-        const double need = (goal - __shfl(incl[half] - m[half], l, kWave)) / keep.fall[pb];
-        need_p = min((uint64_t)fmax(ceil(need), 1.0), in);
+        const double need = (goal - from_lane(incl[half] - m[half], l)) / keep.fall[pb];
+        need_p = min((uint64_t)fmax(ceil(need), 1.0), h.weight[pb]);
       }
     }
   }
@@ -394,7 +409,7 @@ __device__ uint32_t least_of(const Edge& e, const Keep& keep, const float* v, in
   const int tid = threadIdx.x;
   if (n <= kPairs) {
     static_assert(kPairs <= kDigits && kPairs <= NT, "a weight per entry");
-    if (tid < n) digits[tid] = e.need_p ? keep.scale.weight(v[tid], bin) : 0;
+    if (tid < n) digits[tid] = e.need_p ? keep.scale.units(v[tid], bin) : 0;
     if (tid == 0) *least = 0;
     __syncthreads();
     for (int i = tid / 8; i < n; i += NT / 8) {
@@ -426,7 +441,7 @@ __device__ uint32_t least_of(const Edge& e, const Keep& keep, const float* v, in
   auto key = [&](int i) { return order(v[i]); };
   uint32_t k = 0;
   if (e.need_k) k = key_reaching<NT>(n, e.need_k, digits, red, key, [](int) { return 1ull; });
-  if (e.need_p) k = max(k, key_reaching<NT>(n, e.need_p, digits, red, key, [&](int i) { return keep.scale.weight(v[i], bin); }));
+  if (e.need_p) k = max(k, key_reaching<NT>(n, e.need_p, digits, red, key, [&](int i) { return keep.scale.units(v[i], bin); }));
   return k;
 }
 
@@ -477,7 +492,7 @@ struct Histogram {
     if (!(r < kBins)) return;
     const int c = threadIdx.x % kCopies;
     if (counts) atomicAdd(&count[(int)r][c], 1u);
-    if (weights) add_u64(&weight[(int)r][c], s.weight(x, b));
+    if (weights) add_u64(&weight[(int)r][c], s.units(x, b));
   }
   __device__ __forceinline__ void sum(int r, uint64_t& w, uint32_t& n) const {
     w = 0;
@@ -513,7 +528,7 @@ __global__ void __launch_bounds__(kOneThreads) k_one(const SampleRowsArgs a) {
   const float* x = a.logits + (size_t)row * a.ld;
   Row c;
   c.load(x, 0, a.V);
-  if (tid < kBins) fall[tid] = exp(-0.25 * tid);
+  if (tid < kBins) fall[tid] = fall_of(tid);
   if (filtered(a)) sh.h.clear();
   if (tid == 0) n = 0;
   const float mx = from_order(group_max<NT>(c.top(), red));
@@ -524,7 +539,7 @@ __global__ void __launch_bounds__(kOneThreads) k_one(const SampleRowsArgs a) {
   }
   const float u = a.u[row];
   const Scale scale = scale_of(a);
-  Keep keep = {scale, fall, scale.bin(mx), mx, a.min_gap, 0};
+  Keep keep = {scale, fall, scale.bin(mx), mx, a.min_gap, -INFINITY};
   if (!is_near(keep.top)) {
     const int i = slow<NT>(a, x, mx, u, digits, red);
     if (tid == 0) a.out[row] = i;
@@ -547,7 +562,7 @@ __global__ void __launch_bounds__(kOneThreads) k_one(const SampleRowsArgs a) {
       for (int k = 0; k < kOne / NT; ++k)
         if (keep.top - scale.bin(c.x[k]) == (float)e.r) sh.v[atomicAdd(&n, 1)] = c.x[k];
       __syncthreads();
-      keep.least = least_of<NT>(e, keep, sh.v, n, digits, red, &least);
+      keep.least = from_order(least_of<NT>(e, keep, sh.v, n, digits, red, &least));
     }
   }
   const int i = c.pick(keep, 0.0, fraction(u), true, part, red);
@@ -622,7 +637,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   const float* x = a.logits + (size_t)row * a.ld;
   for (int t = tid; t < tiles; t += NT) tops[t] = w.top[t];
   if (tid < kBins) {
-    fall[tid] = exp(-0.25 * tid);
+    fall[tid] = fall_of(tid);
     bins.weight[tid] = 0;
     bins.count[tid] = 0;
   }
@@ -641,7 +656,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   }
   const float u = a.u[row];
   const Scale scale = scale_of(a);
-  Keep keep = {scale, fall, scale.bin(mx), mx, a.min_gap, 0};
+  Keep keep = {scale, fall, scale.bin(mx), mx, a.min_gap, -INFINITY};
   if (!is_near(keep.top)) {
     const int i = slow<NT>(a, x, mx, u, digits, red);
     if (tid == 0) a.out[row] = i;
@@ -692,13 +707,12 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = lane + 64 * h;
-      if (r < e.r) s += (double)weight[k][h] * fall[r];
+      if (r < e.r) s += (double)weight[k][h] * (1.0 / kUnit) * fall[r];
       some = some || (r == e.r && weight[k][h] > 0);
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
+    s = wave_upto(s);
     const bool any = __any(some);
-    if (lane == 0) {
+    if (lane == 63) {
       kept[t] = s;
       edge_kept[t] = 0;
       there[t] = any;
@@ -710,23 +724,39 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
     const float bin = keep.top - (float)e.r;
     for (int i0 = 0; i0 < a.V; i0 += kRounds * 4 * NT) {
       Chunk<NT, 4> c[kRounds];
+      uint32_t hit = 0;   // bit 4k + j
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) {
         const int i = i0 + 4 * k * NT;
         if (i < a.V && there[i / kTile]) c[k].load(x, i, a.V);
+        else c[k].x[0] = c[k].x[1] = c[k].x[2] = c[k].x[3] = -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < kRounds; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) hit |= scale.bin(c[k].x[j]) == bin ? 1u << (4 * k + j) : 0u;
+      if (!__any(hit)) continue;
+      int p = 0;
+      if (e.inside()) {   // room in the list for the wave's
+        const uint64_t mine = __popc(hit), upto = wave_upto(mine);
+        if (lane == 63) p = atomicAdd(&n, (int)upto);
+        p = __builtin_amdgcn_readlane(p, 63) + (int)(upto - mine);
       }
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) {
-        const int i = i0 + 4 * k * NT;
-        if (i >= a.V || !there[i / kTile]) continue;
+        if (!__any(hit >> 4 * k & 15)) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (scale.bin(c[k].x[j]) != bin) continue;
+          if (!(hit >> (4 * k + j) & 1)) continue;
+          const float y = c[k].x[j];
+          const int i = i0 + 4 * k * NT + c[k].at(0, j);
           if (!e.inside()) {
-            if (gap(c[k].x[j], mx) >= a.min_gap) add_u64(&edge_kept[i / kTile], scale.weight(c[k].x[j], bin));
-          } else if (const int p = atomicAdd(&n, 1); p < kList) {
-            v[p] = c[k].x[j];
-            at[p] = i + c[k].at(0, j);
+            if (keep.stays(y)) add_u64(&edge_kept[i / kTile], scale.units(y, bin));
+          } else if (p < kList) {
+            v[p] = y;
+            at[p++] = i;
+          } else {
+            ++p;
           }
         }
       }
@@ -738,12 +768,12 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
       return;
     }
     if (e.inside()) {
-      keep.least = least_of<NT>(e, keep, v, n, digits, red, &least);
+      keep.least = from_order(least_of<NT>(e, keep, v, n, digits, red, &least));
       for (int i = tid; i < n; i += NT)
-        if (keep(v[i]) > 0.0) add_u64(&edge_kept[at[i] / kTile], scale.weight(v[i], bin));
+        if (keep.stays(v[i])) add_u64(&edge_kept[at[i] / kTile], scale.units(v[i], bin));
       __syncthreads();
     }
-    for (int t = tid; t < tiles; t += NT) kept[t] += (double)edge_kept[t] * fall[e.r];
+    for (int t = tid; t < tiles; t += NT) kept[t] += (double)edge_kept[t] * (1.0 / kUnit) * fall[e.r];
     __syncthreads();
   }
   double total = 0.0, before = 0.0;
