@@ -43,9 +43,9 @@ constexpr int kList = 8192;                 // entries of the threshold's bin
 constexpr int kPairs = 256;                 // up to this many are compared each with all
 constexpr float kFar = 1048576.f;           // 2^20 bins from 0: neighbours are not told apart
 
-constexpr int kOneThreads = 1024, kOne = 4 * kOneThreads;
+constexpr int kOneThreads = 1024, kOne = 8 * kOneThreads;   // of 4 or 8 entries each
 constexpr int kTileThreads = 512;           // of 8 or 16 entries each
-constexpr int kRowThreads = 1024, kRounds = 8;   // the row's workgroup goes through rounds of 4096 entries, 8 at a time
+constexpr int kRowThreads = 1024, kRounds = 4;   // the row's workgroup goes through rounds of 4096 entries, 4 at a time
 constexpr int kMaxTiles = (kSampleRowsMaxV + 8 * kTileThreads - 1) / (8 * kTileThreads);   // 128
 
 // unsigned key that orders like the value; NaN as -inf, -0 as 0
@@ -71,11 +71,10 @@ struct Scale {
   double inv;
   __device__ __forceinline__ float bin(float x) const { return x == x ? floorf(x * per) : -INFINITY; }
   // e^(x / T - the middle of bin b), for |x / T - that| of 1/8 and a little: the
-  // ninth power's term is below 2e-13
+  // eighth power's term is below 2e-12
   __device__ __forceinline__ double weight(float x, float b) const {
-    const double r = fma((double)x, inv, -0.25 * ((double)b + 0.5));
-    double p = 1.0 / 40320;
-    p = fma(p, r, 1.0 / 5040);
+    const double r = fma((double)x, inv, (double)fmaf(b, -0.25f, -0.125f));
+    double p = 1.0 / 5040;
     p = fma(p, r, 1.0 / 720);
     p = fma(p, r, 1.0 / 120);
     p = fma(p, r, 1.0 / 24);
@@ -237,17 +236,21 @@ __device__ __forceinline__ double fall_of(int r) {
 struct Keep {
   Scale scale;
   const double* fall;   // fall_of(r), r < kBins
-  float top, mx;        // the maximum's bin and the maximum
-  double min_gap;
-  float least;          // the least that stays by top-k and top-p
-  __device__ __forceinline__ bool stays(float x) const {   // (not a NaN; entries of 0 weight aside)
-    return x >= least && (min_gap == -INFINITY || gap(x, mx) >= min_gap);
-  }
+  float top;            // the maximum's bin
+  float least;          // the least that stays
   __device__ __forceinline__ double operator()(float x) const {
     const float b = scale.bin(x), r = top - b;
-    return r < kBins && stays(x) ? scale.weight(x, b) * fall[(int)r] : 0.0;
+    return r < kBins && x >= least ? scale.weight(x, b) * fall[(int)r] : 0.0;
   }
 };
+// the least float that stays by min-p
+__device__ __forceinline__ float least_by_gap(float mx, double min_gap) {
+  if (min_gap == -INFINITY) return -INFINITY;
+  uint32_t k = order((float)((double)mx + min_gap));
+  while (gap(from_order(k), mx) < min_gap) ++k;        // (a step at most: the sum rounds to the nearest float)
+  while (gap(from_order(k - 1), mx) >= min_gap) --k;
+  return from_order(k);
+}
 
 // ---- a row's entries in the registers of a workgroup ---------------------------
 // x[4k + j] of thread t is entry 4 (k * NT + t) + j of those loaded (-inf past the row)
@@ -268,11 +271,11 @@ struct Chunk {
       }
     }
   }
-  __device__ __forceinline__ uint32_t top() const {
-    uint32_t m = 0;
+  __device__ __forceinline__ uint32_t top() const {   // the maximum's key
+    float m = -INFINITY;   // (fmaxf leaves a NaN aside)
 #pragma unroll
-    for (int e = 0; e < E; ++e) m = max(m, order(x[e]));
-    return m;
+    for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
+    return order(m);
   }
   // the first index of value v
   __device__ int first(float v, uint64_t* red) const {
@@ -391,9 +394,9 @@ __device__ __forceinline__ Edge find_edge(const SampleRowsArgs& a, const Bins& h
       }
     }
   }
-  if (keep.min_gap > -INFINITY) {
-    const float r = keep.top - keep.scale.bin((float)((double)keep.mx + keep.min_gap));
-    mb = r < kBins ? (int)fmaxf(r, 0.f) : kBins;
+  if (keep.least > -INFINITY) {   // min-p's
+    const float r = keep.top - keep.scale.bin(keep.least);
+    mb = r < kBins ? (int)r : kBins;
   }
   const int r = min(min(kb, pb), mb);
   return {r, kb == r ? need_k : 0, pb == r ? need_p : 0};
@@ -511,12 +514,13 @@ __device__ __forceinline__ bool filtered(const SampleRowsArgs& a) { return a.top
 __device__ __forceinline__ bool is_near(float top) { return top > -kFar && top < kFar; }
 
 // ---- one workgroup per row ---------------------------------------------------------
+template <int E>
 __global__ void __launch_bounds__(kOneThreads) k_one(const SampleRowsArgs a) {
   constexpr int NT = kOneThreads;
-  using Row = Chunk<NT, kOne / NT>;
+  using Row = Chunk<NT, E>;
   __shared__ union {
     Histogram<NT> h;
-    float v[kOne];
+    float v[NT * E];
   } sh;
   __shared__ Bins bins;
   __shared__ double fall[kBins], part[Row::kRounds * NT / 64];
@@ -539,15 +543,16 @@ __global__ void __launch_bounds__(kOneThreads) k_one(const SampleRowsArgs a) {
   }
   const float u = a.u[row];
   const Scale scale = scale_of(a);
-  Keep keep = {scale, fall, scale.bin(mx), mx, a.min_gap, -INFINITY};
+  Keep keep = {scale, fall, scale.bin(mx), -INFINITY};
   if (!is_near(keep.top)) {
     const int i = slow<NT>(a, x, mx, u, digits, red);
     if (tid == 0) a.out[row] = i;
     return;
   }
+  keep.least = least_by_gap(mx, a.min_gap);
   if (filtered(a)) {
 #pragma unroll
-    for (int e = 0; e < kOne / NT; ++e) sh.h.add(c.x[e], keep.top, scale, a.top_k, a.top_p < 1.0);
+    for (int e = 0; e < E; ++e) sh.h.add(c.x[e], keep.top, scale, a.top_k, a.top_p < 1.0);
     __syncthreads();
     if (tid < kBins) sh.h.sum(tid, bins.weight[tid], bins.count[tid]);
     __syncthreads();
@@ -559,10 +564,10 @@ __global__ void __launch_bounds__(kOneThreads) k_one(const SampleRowsArgs a) {
     const Edge e = edge;
     if (e.inside()) {   // (else min-p alone cuts there, and the entries are asked one by one)
 #pragma unroll
-      for (int k = 0; k < kOne / NT; ++k)
+      for (int k = 0; k < E; ++k)
         if (keep.top - scale.bin(c.x[k]) == (float)e.r) sh.v[atomicAdd(&n, 1)] = c.x[k];
       __syncthreads();
-      keep.least = from_order(least_of<NT>(e, keep, sh.v, n, digits, red, &least));
+      keep.least = fmaxf(keep.least, from_order(least_of<NT>(e, keep, sh.v, n, digits, red, &least)));
     }
   }
   const int i = c.pick(keep, 0.0, fraction(u), true, part, red);
@@ -656,12 +661,13 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   }
   const float u = a.u[row];
   const Scale scale = scale_of(a);
-  Keep keep = {scale, fall, scale.bin(mx), mx, a.min_gap, -INFINITY};
+  Keep keep = {scale, fall, scale.bin(mx), -INFINITY};
   if (!is_near(keep.top)) {
     const int i = slow<NT>(a, x, mx, u, digits, red);
     if (tid == 0) a.out[row] = i;
     return;
   }
+  keep.least = least_by_gap(mx, a.min_gap);
   // the tiles' bins, tile t in wave t % 16, bins lane and 64 + lane of the row's;
   // a tile's own begin `shift` bins further down
   uint64_t weight[kMost][2];
@@ -720,46 +726,42 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   }
   __syncthreads();
   if (e.r < kBins) {
-    // that bin's entries: into the list, or, where min-p alone cuts, those that pass
+    // that bin's entries: their places into the list, the next rounds' entries
+    // requested before these are looked at
     const float bin = keep.top - (float)e.r;
-    for (int i0 = 0; i0 < a.V; i0 += kRounds * 4 * NT) {
-      Chunk<NT, 4> c[kRounds];
-      uint32_t hit = 0;   // bit 4k + j
+    using Round = Chunk<NT, 4>;
+    Round c[2][kRounds];
+    auto load = [&](Round (&d)[kRounds], int i0) {
 #pragma unroll
       for (int k = 0; k < kRounds; ++k) {
         const int i = i0 + 4 * k * NT;
-        if (i < a.V && there[i / kTile]) c[k].load(x, i, a.V);
-        else c[k].x[0] = c[k].x[1] = c[k].x[2] = c[k].x[3] = -INFINITY;
+        if (i < a.V && there[i / kTile]) d[k].load(x, i, a.V);
+        else d[k].x[0] = d[k].x[1] = d[k].x[2] = d[k].x[3] = -INFINITY;
       }
+    };
+    auto look = [&](const Round (&d)[kRounds], int i0) {
+      uint32_t hit = 0;   // bit 4k + j
 #pragma unroll
       for (int k = 0; k < kRounds; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) hit |= scale.bin(c[k].x[j]) == bin ? 1u << (4 * k + j) : 0u;
-      if (!__any(hit)) continue;
+        for (int j = 0; j < 4; ++j) hit |= scale.bin(d[k].x[j]) == bin ? 1u << (4 * k + j) : 0u;
+      if (!__any(hit)) return;
+      const uint64_t mine = __popc(hit), upto = wave_upto(mine);
       int p = 0;
-      if (e.inside()) {   // room in the list for the wave's
-        const uint64_t mine = __popc(hit), upto = wave_upto(mine);
-        if (lane == 63) p = atomicAdd(&n, (int)upto);
-        p = __builtin_amdgcn_readlane(p, 63) + (int)(upto - mine);
+      if (lane == 63) p = atomicAdd(&n, (int)upto);   // room for the wave's
+      p = __builtin_amdgcn_readlane(p, 63) + (int)(upto - mine);
+      for (; hit; hit &= hit - 1, ++p) {
+        const int b = __ffs(hit) - 1;
+        if (p < kList) at[p] = i0 + 4 * (b / 4) * NT + Round::at(0, b % 4);
       }
-#pragma unroll
-      for (int k = 0; k < kRounds; ++k) {
-        if (!__any(hit >> 4 * k & 15)) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (!(hit >> (4 * k + j) & 1)) continue;
-          const float y = c[k].x[j];
-          const int i = i0 + 4 * k * NT + c[k].at(0, j);
-          if (!e.inside()) {
-            if (keep.stays(y)) add_u64(&edge_kept[i / kTile], scale.units(y, bin));
-          } else if (p < kList) {
-            v[p] = y;
-            at[p++] = i;
-          } else {
-            ++p;
-          }
-        }
-      }
+    };
+    constexpr int kStep = 4 * kRounds * NT;
+    load(c[0], 0);
+    for (int i0 = 0; i0 < a.V; i0 += 2 * kStep) {
+      load(c[1], i0 + kStep);
+      look(c[0], i0);
+      load(c[0], i0 + 2 * kStep);
+      look(c[1], i0 + kStep);
     }
     __syncthreads();
     if (n > kList) {
@@ -767,12 +769,13 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
       if (tid == 0) a.out[row] = i;
       return;
     }
-    if (e.inside()) {
-      keep.least = from_order(least_of<NT>(e, keep, v, n, digits, red, &least));
-      for (int i = tid; i < n; i += NT)
-        if (keep.stays(v[i])) add_u64(&edge_kept[at[i] / kTile], scale.units(v[i], bin));
-      __syncthreads();
-    }
+    for (int i = tid; i < n; i += NT) v[i] = x[at[i]];
+    __syncthreads();
+    if (e.inside())   // (else min-p alone cuts there)
+      keep.least = fmaxf(keep.least, from_order(least_of<NT>(e, keep, v, n, digits, red, &least)));
+    for (int i = tid; i < n; i += NT)
+      if (v[i] >= keep.least) add_u64(&edge_kept[at[i] / kTile], scale.units(v[i], bin));
+    __syncthreads();
     for (int t = tid; t < tiles; t += NT) kept[t] += (double)edge_kept[t] * (1.0 / kUnit) * fall[e.r];
     __syncthreads();
   }
@@ -821,7 +824,10 @@ hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s) {
   if (a.rows < 1 || a.V < 1 || a.V > kSampleRowsMaxV) return hipErrorInvalidValue;
   if (const int tiles = tiles_of(a.rows, a.V, a.n_cu))
     return entries_of(a.rows, a.V, a.n_cu) == 8 ? launch_tiles<8>(a, tiles, s) : launch_tiles<16>(a, tiles, s);
-  hipLaunchKernelGGL(k_one, dim3(a.rows), dim3(kOneThreads), 0, s, a);
+  if (a.V <= 4 * kOneThreads)
+    hipLaunchKernelGGL(k_one<4>, dim3(a.rows), dim3(kOneThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(k_one<8>, dim3(a.rows), dim3(kOneThreads), 0, s, a);
   return hipGetLastError();
 }
 
