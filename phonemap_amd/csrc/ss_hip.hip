@@ -827,7 +827,7 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, con
 
 size_t ss_hip_sample_rows_workspace(ss_hip_ctx_t* c, int32_t n_rows, int32_t n) {
   if (!c || n_rows <= 0 || n_rows > 65535 || n <= 0 || n > ssk::kSampleRowsMaxV) return 0;
-  return ssk::sample_rows_workspace(n_rows, n, c->n_cu);
+  return ssk::sample_rows_workspace(n_rows, n);
 }
 
 int32_t ss_hip_sample_rows(ss_hip_ctx_t* c, int32_t* out, const float* logits, int32_t n, int32_t n_rows, int64_t ld,
@@ -851,7 +851,7 @@ int32_t ss_hip_sample_rows(ss_hip_ctx_t* c, int32_t* out, const float* logits, i
   a.top_k = top_k > 0 && top_k < n ? top_k : 0;
   a.top_p = top_p > 0.f && top_p < 1.f ? top_p : 1.0;
   a.min_gap = a.temperature > 0.0 && min_p > 0.f ? a.temperature * log((double)min_p) : -INFINITY;
-  if (int32_t rc = check_scratch("sample_rows", ws, ws_bytes, ssk::sample_rows_workspace(n_rows, n, c->n_cu))) return rc;
+  if (int32_t rc = check_scratch("sample_rows", ws, ws_bytes, ssk::sample_rows_workspace(n_rows, n))) return rc;
   a.work = ws;
   a.n_cu = c->n_cu;
   DeviceScope on(c->device);

@@ -307,7 +307,7 @@ struct SampleRowsArgs {
   int n_cu;                  // compute units
 };
 constexpr int kSampleRowsMaxV = (1 << 19) - 1;   // sums of weights up to 2^44 stay below 2^63
-size_t sample_rows_workspace(int rows, int V, int n_cu);
+size_t sample_rows_workspace(int rows, int V);
 hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s);
 hipError_t launch_set_state(int* dpos, int* tokens, int pos, int token, hipStream_t s);
 hipError_t launch_advance(int* dpos, hipStream_t s);

@@ -23,10 +23,12 @@
 // 2^18, leaves the row to `slow`, which selects by the bits of x over the whole row.
 //
 // Rows of up to kOne entries: one workgroup with the row in registers, one launch.
-// Longer ones: a launch over tiles for their maxima and histograms, and one with a
-// workgroup per row, which adds up the bins, goes through the tiles that have
-// entries in the threshold's bin, and draws within one tile. Weights are formed
-// once, for the histogram, and again for the threshold's bin and the last tile.
+// Longer ones: a launch over tiles for their maxima and histograms, and one with
+// some workgroups per row, each of which adds up the bins and goes through a part
+// of the tiles that have entries in the threshold's bin; the last of a row to
+// finish (by a count that the first launch clears) finds the threshold and draws
+// within one tile. Weights are formed once, for the histogram, and again for the
+// threshold's bin and the last tile.
 
 #include <type_traits>
 
@@ -44,9 +46,10 @@ constexpr int kPairs = 256;                 // up to this many are compared each
 constexpr float kFar = 1048576.f;           // 2^20 bins from 0: neighbours are not told apart
 
 constexpr int kOneThreads = 1024, kOne = 8 * kOneThreads;   // of 4 or 8 entries each
-constexpr int kTileThreads = 512;           // of 8 or 16 entries each
+constexpr int kTileThreads = 512, kTileEach = 8, kTile = kTileThreads * kTileEach;
+constexpr int kMaxTiles = (kSampleRowsMaxV + kTile - 1) / kTile;   // 128
 constexpr int kRowThreads = 1024, kRounds = 4;   // the row's workgroup goes through rounds of 4096 entries, 4 at a time
-constexpr int kMaxTiles = (kSampleRowsMaxV + 8 * kTileThreads - 1) / (8 * kTileThreads);   // 128
+constexpr int kStep = 4 * kRounds * kRowThreads;
 
 // unsigned key that orders like the value; NaN as -inf, -0 as 0
 __device__ __forceinline__ uint32_t order(float x) {
@@ -187,30 +190,29 @@ __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_
   const uint32_t first = key(0);
   uint32_t differ = 0;
   for (int i = threadIdx.x; i < n; i += NT) differ |= key(i) ^ first;
-  differ = group_max<NT>(differ ? 32 - __clz((int)differ) : 0, red);   // as many low bits do not
-  int shift = (int)differ;
+  for (int d = threadIdx.x; d < kDigits; d += NT) hist[d] = 0;
+  int shift = (int)group_max<NT>(differ ? 32 - __clz((int)differ) : 0, red);   // as many low bits do not
+  uint64_t* found = red + NT / 64;
   uint32_t mask = shift < 32 ? ~0u << shift : 0u, prefix = first & mask;
   uint64_t above = 0;
   do {
     const int bits = min(kDigit, shift);
     shift -= bits;
     const uint32_t digit = (1u << bits) - 1;
-    __syncthreads();
-    if (threadIdx.x < kDigits) hist[threadIdx.x] = 0;
-    __syncthreads();
     for (int i = threadIdx.x; i < n; i += NT) {
       const uint32_t k = key(i);
       if ((k & mask) == prefix) add_u64(&hist[(k >> shift) & digit], val(i));
     }
-    __syncthreads();
-    const uint64_t h = threadIdx.x < kDigits ? hist[kDigits - 1 - threadIdx.x] : 0;   // thread 0 has the highest digit
-    uint64_t all;
-    const uint64_t before = above + sum_before<NT>(h, red, all);
-    uint64_t* found = red + NT / 64;
     if (threadIdx.x == 0) found[0] = kDigits;
     __syncthreads();
-    if (threadIdx.x < kDigits && before < target && before + h >= target) {
-      found[0] = kDigits - 1 - threadIdx.x;
+    // thread 0 has the highest digit; its bin is clear for the next digit
+    const int d = kDigits - 1 - (int)threadIdx.x;
+    const uint64_t h = d >= 0 ? hist[d] : 0;
+    if (d >= 0) hist[d] = 0;
+    uint64_t all;
+    const uint64_t before = above + sum_before<NT>(h, red, all);
+    if (before < target && before + h >= target) {
+      found[0] = d;
       found[1] = before;
     }
     __syncthreads();
@@ -218,6 +220,7 @@ __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_
     prefix |= (uint32_t)found[0] << shift;
     mask |= digit << shift;
     above = found[1];
+    __syncthreads();
   } while (shift > 0);
   return prefix;
 }
@@ -579,6 +582,8 @@ struct RowWork {
   Bins* bins;          // [tiles], each from its own maximum's bin down
   uint32_t* top;       // [tiles] the maximum's key
   int* first;          // [tiles] temperature 0: its first index
+  uint32_t* list;      // [kList] places of the threshold's bin's entries
+  uint32_t* count;     // [0] as many, [1] workgroups done
 };
 __host__ __device__ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 __host__ __device__ inline RowWork row_work(void* work, int row, int tiles, size_t* bytes) {
@@ -588,30 +593,34 @@ __host__ __device__ inline RowWork row_work(void* work, int row, int tiles, size
     o += up256(n);
     return at;
   };
-  const size_t b = take(sizeof(Bins) * tiles), t = take(sizeof(uint32_t) * tiles), f = take(sizeof(int) * tiles);
+  const size_t b = take(sizeof(Bins) * tiles), t = take(sizeof(uint32_t) * tiles), f = take(sizeof(int) * tiles),
+               l = take(sizeof(uint32_t) * kList), c = take(2 * sizeof(uint32_t));
   uint8_t* p = static_cast<uint8_t*>(work) + (size_t)row * o;
   if (bytes) *bytes = o;
-  return {reinterpret_cast<Bins*>(p + b), reinterpret_cast<uint32_t*>(p + t), reinterpret_cast<int*>(p + f)};
+  return {reinterpret_cast<Bins*>(p + b), reinterpret_cast<uint32_t*>(p + t), reinterpret_cast<int*>(p + f),
+          reinterpret_cast<uint32_t*>(p + l), reinterpret_cast<uint32_t*>(p + c)};
 }
 
 // 1. a tile's maximum and bins. Grid: tiles x rows.
-template <int E>
 __global__ void __launch_bounds__(kTileThreads) k_tiles(const SampleRowsArgs a) {
-  constexpr int NT = kTileThreads;
+  constexpr int NT = kTileThreads, E = kTileEach;
   __shared__ Histogram<NT> h;
   __shared__ uint64_t red[NT / 64 + 2];
   const int tid = threadIdx.x, tile = blockIdx.x, row = blockIdx.y;
   const RowWork w = row_work(a.work, row, gridDim.x, nullptr);
   Chunk<NT, E> c;
-  c.load(a.logits + (size_t)row * a.ld, tile * NT * E, a.V);
+  c.load(a.logits + (size_t)row * a.ld, tile * kTile, a.V);
   h.clear();
   const uint32_t mk = group_max<NT>(c.top(), red);
-  if (tid == 0) w.top[tile] = mk;
+  if (tid == 0) {
+    w.top[tile] = mk;
+    if (tile == 0) w.count[0] = w.count[1] = 0;
+  }
   const float mx = from_order(mk);
   if (mx == -INFINITY) return;
   if (!(a.temperature > 0.0)) {
     const int i = c.first(mx, red);
-    if (tid == 0) w.first[tile] = tile * NT * E + i;
+    if (tid == 0) w.first[tile] = tile * kTile + i;
     return;
   }
   const Scale scale = scale_of(a);
@@ -622,11 +631,10 @@ __global__ void __launch_bounds__(kTileThreads) k_tiles(const SampleRowsArgs a) 
   if (tid < kBins) h.sum(tid, w.bins[tile].weight[tid], w.bins[tile].count[tid]);
 }
 
-// 2. threshold and token. Grid: rows.
-template <int E>
+// 2. threshold and token. Grid: workgroups of a row x rows.
 __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, int tiles) {
-  constexpr int NT = kRowThreads, kTile = kTileThreads * E, kWaves = NT / 64;
-  constexpr int kMost = (kMaxTiles * 8 / E + kWaves - 1) / kWaves;   // tiles of a wave
+  constexpr int NT = kRowThreads, kWaves = NT / 64;
+  constexpr int kMost = (kMaxTiles + kWaves - 1) / kWaves;   // tiles of a wave
   using Tile = Chunk<NT, kTile / NT>;
   __shared__ float v[kList];
   __shared__ int at[kList];
@@ -635,9 +643,11 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   __shared__ uint64_t red[kWaves + 2], digits[kDigits], edge_kept[kMaxTiles];
   __shared__ uint32_t tops[kMaxTiles], least;
   __shared__ int n;
+  __shared__ uint32_t base, done;
   __shared__ bool there[kMaxTiles];   // the tile has entries in the threshold's bin
   __shared__ Edge edge;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y;
+  const int share = blockIdx.x, shares = gridDim.x;
   const RowWork w = row_work(a.work, row, tiles, nullptr);
   const float* x = a.logits + (size_t)row * a.ld;
   for (int t = tid; t < tiles; t += NT) tops[t] = w.top[t];
@@ -652,7 +662,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   for (int t = 0; t < tiles; ++t) mk = max(mk, tops[t]);
   const float mx = from_order(mk);
   if (mx == -INFINITY || !(a.temperature > 0.0)) {   // nothing to choose from, or the first maximum
-    if (tid == 0) {
+    if (share == 0 && tid == 0) {
       int t = 0;
       while (tops[t] != mk) ++t;
       a.out[row] = mx == -INFINITY ? -1 : w.first[t];
@@ -663,6 +673,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   const Scale scale = scale_of(a);
   Keep keep = {scale, fall, scale.bin(mx), -INFINITY};
   if (!is_near(keep.top)) {
+    if (share) return;
     const int i = slow<NT>(a, x, mx, u, digits, red);
     if (tid == 0) a.out[row] = i;
     return;
@@ -725,6 +736,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
     }
   }
   __syncthreads();
+  if (e.r == kBins && share) return;
   if (e.r < kBins) {
     // that bin's entries: their places into the list, the next rounds' entries
     // requested before these are looked at
@@ -755,15 +767,31 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
         if (p < kList) at[p] = i0 + 4 * (b / 4) * NT + Round::at(0, b % 4);
       }
     };
-    constexpr int kStep = 4 * kRounds * NT;
-    load(c[0], 0);
-    for (int i0 = 0; i0 < a.V; i0 += 2 * kStep) {
-      load(c[1], i0 + kStep);
+    const int step = kStep * shares;
+    load(c[0], kStep * share);
+    for (int i0 = kStep * share; i0 < a.V; i0 += 2 * step) {
+      load(c[1], i0 + step);
       look(c[0], i0);
-      load(c[0], i0 + 2 * kStep);
-      look(c[1], i0 + kStep);
+      load(c[0], i0 + 2 * step);
+      look(c[1], i0 + step);
     }
     __syncthreads();
+    if (shares > 1) {   // the row's list, from its workgroups' parts
+      if (tid == 0) base = n ? __hip_atomic_fetch_add(&w.count[0], (uint32_t)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
+      __syncthreads();
+      for (int i = tid; i < min(n, kList); i += NT)
+        if (base + i < (uint32_t)kList) cst(&w.list[base + i], (uint32_t)at[i]);
+      vm_drain();   // what this wave published
+      __syncthreads();
+      if (tid == 0) {
+        done = __hip_atomic_fetch_add(&w.count[1], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+        if (done == (uint32_t)shares) n = (int)cld(&w.count[0]);
+      }
+      __syncthreads();
+      if (done != (uint32_t)shares) return;
+      for (int i = tid; i < min(n, kList); i += NT) at[i] = (int)cld(&w.list[i]);
+      __syncthreads();
+    }
     if (n > kList) {
       const int i = slow<NT>(a, x, mx, u, digits, red);
       if (tid == 0) a.out[row] = i;
@@ -794,40 +822,31 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   if (tid == 0) a.out[row] = t * kTile + i;
 }
 
-// entries a thread of the tiles has: 8 where that gives a workgroup for every two
-// compute units at most
-int entries_of(int rows, int V, int n_cu) {
-  return (int64_t)rows * ((V + 8 * kTileThreads - 1) / (8 * kTileThreads)) * 2 <= n_cu ? 8 : 16;
-}
-int tiles_of(int rows, int V, int n_cu) {
-  const int tile = entries_of(rows, V, n_cu) * kTileThreads;
-  return V <= kOne ? 0 : (V + tile - 1) / tile;
-}
-
-template <int E>
-hipError_t launch_tiles(const SampleRowsArgs& a, int tiles, hipStream_t s) {
-  const dim3 grid(tiles, a.rows), block(kTileThreads);
-  hipLaunchKernelGGL(k_tiles<E>, grid, block, 0, s, a);
-  hipLaunchKernelGGL(k_draw<E>, dim3(a.rows), dim3(kRowThreads), 0, s, a, tiles);
-  return hipGetLastError();
+int tiles_of(int V) { return V <= kOne ? 0 : (V + kTile - 1) / kTile; }
+// workgroups of a row in the second launch
+int shares_of(int rows, int V, int n_cu) {
+  const int steps = (V + kStep - 1) / kStep, room = n_cu / rows;
+  return steps < 4 || room < 2 ? 1 : steps < room ? steps : room;
 }
 
 }  // namespace
 
-size_t sample_rows_workspace(int rows, int V, int n_cu) {
+size_t sample_rows_workspace(int rows, int V) {
   size_t bytes = 0;
-  if (const int tiles = tiles_of(rows, V, n_cu)) row_work(nullptr, 0, tiles, &bytes);
+  if (const int tiles = tiles_of(V)) row_work(nullptr, 0, tiles, &bytes);
   return bytes * rows;
 }
 
 hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s) {
   if (a.rows < 1 || a.V < 1 || a.V > kSampleRowsMaxV) return hipErrorInvalidValue;
-  if (const int tiles = tiles_of(a.rows, a.V, a.n_cu))
-    return entries_of(a.rows, a.V, a.n_cu) == 8 ? launch_tiles<8>(a, tiles, s) : launch_tiles<16>(a, tiles, s);
-  if (a.V <= 4 * kOneThreads)
+  if (const int tiles = tiles_of(a.V)) {
+    hipLaunchKernelGGL(k_tiles, dim3(tiles, a.rows), dim3(kTileThreads), 0, s, a);
+    hipLaunchKernelGGL(k_draw, dim3(shares_of(a.rows, a.V, a.n_cu), a.rows), dim3(kRowThreads), 0, s, a, tiles);
+  } else if (a.V <= 4 * kOneThreads) {
     hipLaunchKernelGGL(k_one<4>, dim3(a.rows), dim3(kOneThreads), 0, s, a);
-  else
+  } else {
     hipLaunchKernelGGL(k_one<8>, dim3(a.rows), dim3(kOneThreads), 0, s, a);
+  }
   return hipGetLastError();
 }
 
