@@ -45,10 +45,10 @@ constexpr int kList = 8192;                 // entries of the threshold's bin
 constexpr int kPairs = 256;                 // up to this many are compared each with all
 constexpr float kFar = 1048576.f;           // 2^20 bins from 0: neighbours are not told apart
 
-constexpr int kOneThreads = 1024, kOne = 8 * kOneThreads;   // of 4 or 8 entries each
+constexpr int kOneThreads = 512, kOne = 16 * kOneThreads;   // of 8 or 16 entries each
 constexpr int kTileThreads = 512, kTileEach = 8, kTile = kTileThreads * kTileEach;
 constexpr int kMaxTiles = (kSampleRowsMaxV + kTile - 1) / kTile;   // 128
-constexpr int kRowThreads = 1024, kRounds = 4;   // the row's workgroup goes through rounds of 4096 entries, 4 at a time
+constexpr int kRowThreads = 512, kRounds = 8;   // the row's workgroups go through rounds of 2048 entries, 8 at a time
 constexpr int kStep = 4 * kRounds * kRowThreads;
 
 // unsigned key that orders like the value; NaN as -inf, -0 as 0
@@ -185,7 +185,8 @@ __device__ __forceinline__ void add_u64(uint64_t* p, uint64_t v) {
 constexpr int kDigit = 10, kDigits = 1 << kDigit;
 template <int NT, class Key, class Val>
 __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_t* red, Key key, Val val) {
-  static_assert(NT >= kDigits, "a digit per thread");
+  constexpr int kEach = kDigits / NT;   // digits of a thread, the highest ones in thread 0
+  static_assert(kEach * NT == kDigits, "whole");
   // the bits that all keys share
   const uint32_t first = key(0);
   uint32_t differ = 0;
@@ -205,15 +206,22 @@ __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_
     }
     if (threadIdx.x == 0) found[0] = kDigits;
     __syncthreads();
-    // thread 0 has the highest digit; its bin is clear for the next digit
-    const int d = kDigits - 1 - (int)threadIdx.x;
-    const uint64_t h = d >= 0 ? hist[d] : 0;
-    if (d >= 0) hist[d] = 0;
-    uint64_t all;
-    const uint64_t before = above + sum_before<NT>(h, red, all);
-    if (before < target && before + h >= target) {
-      found[0] = d;
-      found[1] = before;
+    uint64_t h[kEach], sum = 0, all;
+#pragma unroll
+    for (int c = 0; c < kEach; ++c) {
+      const int d = kDigits - 1 - (kEach * (int)threadIdx.x + c);
+      h[c] = hist[d];
+      hist[d] = 0;   // for the next digit
+      sum += h[c];
+    }
+    uint64_t before = above + sum_before<NT>(sum, red, all);
+#pragma unroll
+    for (int c = 0; c < kEach; ++c) {
+      if (before < target && before + h[c] >= target) {
+        found[0] = kDigits - 1 - (kEach * (int)threadIdx.x + c);
+        found[1] = before;
+      }
+      before += h[c];
     }
     __syncthreads();
     if (found[0] == kDigits) return 0;
@@ -582,7 +590,7 @@ struct RowWork {
   Bins* bins;          // [tiles], each from its own maximum's bin down
   uint32_t* top;       // [tiles] the maximum's key
   int* first;          // [tiles] temperature 0: its first index
-  uint32_t* list;      // [kList] places of the threshold's bin's entries
+  uint64_t* list;      // [kList] the threshold's bin's entries: place << 32 | x
   uint32_t* count;     // [0] as many, [1] workgroups done
 };
 __host__ __device__ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -594,11 +602,11 @@ __host__ __device__ inline RowWork row_work(void* work, int row, int tiles, size
     return at;
   };
   const size_t b = take(sizeof(Bins) * tiles), t = take(sizeof(uint32_t) * tiles), f = take(sizeof(int) * tiles),
-               l = take(sizeof(uint32_t) * kList), c = take(2 * sizeof(uint32_t));
+               l = take(sizeof(uint64_t) * kList), c = take(2 * sizeof(uint32_t));
   uint8_t* p = static_cast<uint8_t*>(work) + (size_t)row * o;
   if (bytes) *bytes = o;
   return {reinterpret_cast<Bins*>(p + b), reinterpret_cast<uint32_t*>(p + t), reinterpret_cast<int*>(p + f),
-          reinterpret_cast<uint32_t*>(p + l), reinterpret_cast<uint32_t*>(p + c)};
+          reinterpret_cast<uint64_t*>(p + l), reinterpret_cast<uint32_t*>(p + c)};
 }
 
 // 1. a tile's maximum and bins. Grid: tiles x rows.
@@ -632,9 +640,9 @@ __global__ void __launch_bounds__(kTileThreads) k_tiles(const SampleRowsArgs a) 
 }
 
 // 2. threshold and token. Grid: workgroups of a row x rows.
+template <int kMost>   // tiles of a wave, at most
 __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, int tiles) {
   constexpr int NT = kRowThreads, kWaves = NT / 64;
-  constexpr int kMost = (kMaxTiles + kWaves - 1) / kWaves;   // tiles of a wave
   using Tile = Chunk<NT, kTile / NT>;
   __shared__ float v[kList];
   __shared__ int at[kList];
@@ -679,7 +687,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
     return;
   }
   keep.least = least_by_gap(mx, a.min_gap);
-  // the tiles' bins, tile t in wave t % 16, bins lane and 64 + lane of the row's;
+  // the tiles' bins, tile t in wave t % kWaves, bins lane and 64 + lane of the row's;
   // a tile's own begin `shift` bins further down
   uint64_t weight[kMost][2];
   uint32_t count[kMost][2];
@@ -776,11 +784,13 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
       look(c[1], i0 + step);
     }
     __syncthreads();
+    for (int i = tid; i < min(n, kList); i += NT) v[i] = x[at[i]];
+    __syncthreads();
     if (shares > 1) {   // the row's list, from its workgroups' parts
       if (tid == 0) base = n ? __hip_atomic_fetch_add(&w.count[0], (uint32_t)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
       __syncthreads();
       for (int i = tid; i < min(n, kList); i += NT)
-        if (base + i < (uint32_t)kList) cst(&w.list[base + i], (uint32_t)at[i]);
+        if (base + i < (uint32_t)kList) cst64(&w.list[base + i], (uint64_t)(uint32_t)at[i] << 32 | __float_as_uint(v[i]));
       vm_drain();   // what this wave published
       __syncthreads();
       if (tid == 0) {
@@ -789,7 +799,11 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
       }
       __syncthreads();
       if (done != (uint32_t)shares) return;
-      for (int i = tid; i < min(n, kList); i += NT) at[i] = (int)cld(&w.list[i]);
+      for (int i = tid; i < min(n, kList); i += NT) {
+        const uint64_t y = cld64(&w.list[i]);
+        at[i] = (int)(y >> 32);
+        v[i] = __uint_as_float((uint32_t)y);
+      }
       __syncthreads();
     }
     if (n > kList) {
@@ -797,8 +811,6 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
       if (tid == 0) a.out[row] = i;
       return;
     }
-    for (int i = tid; i < n; i += NT) v[i] = x[at[i]];
-    __syncthreads();
     if (e.inside())   // (else min-p alone cuts there)
       keep.least = fmaxf(keep.least, from_order(least_of<NT>(e, keep, v, n, digits, red, &least)));
     for (int i = tid; i < n; i += NT)
@@ -825,7 +837,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
 int tiles_of(int V) { return V <= kOne ? 0 : (V + kTile - 1) / kTile; }
 // workgroups of a row in the second launch
 int shares_of(int rows, int V, int n_cu) {
-  const int steps = (V + kStep - 1) / kStep, room = n_cu / rows;
+  const int steps = (V + kStep - 1) / kStep, room = 2 * n_cu / rows;
   return steps < 4 || room < 2 ? 1 : steps < room ? steps : room;
 }
 
@@ -841,11 +853,17 @@ hipError_t launch_sample_rows(const SampleRowsArgs& a, hipStream_t s) {
   if (a.rows < 1 || a.V < 1 || a.V > kSampleRowsMaxV) return hipErrorInvalidValue;
   if (const int tiles = tiles_of(a.V)) {
     hipLaunchKernelGGL(k_tiles, dim3(tiles, a.rows), dim3(kTileThreads), 0, s, a);
-    hipLaunchKernelGGL(k_draw, dim3(shares_of(a.rows, a.V, a.n_cu), a.rows), dim3(kRowThreads), 0, s, a, tiles);
-  } else if (a.V <= 4 * kOneThreads) {
-    hipLaunchKernelGGL(k_one<4>, dim3(a.rows), dim3(kOneThreads), 0, s, a);
-  } else {
+    const dim3 grid(shares_of(a.rows, a.V, a.n_cu), a.rows), block(kRowThreads);
+    if (tiles <= 16)
+      hipLaunchKernelGGL(k_draw<2>, grid, block, 0, s, a, tiles);
+    else if (tiles <= 32)
+      hipLaunchKernelGGL(k_draw<4>, grid, block, 0, s, a, tiles);
+    else
+      hipLaunchKernelGGL(k_draw<kMaxTiles * 64 / kRowThreads>, grid, block, 0, s, a, tiles);
+  } else if (a.V <= 8 * kOneThreads) {
     hipLaunchKernelGGL(k_one<8>, dim3(a.rows), dim3(kOneThreads), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(k_one<16>, dim3(a.rows), dim3(kOneThreads), 0, s, a);
   }
   return hipGetLastError();
 }
