@@ -184,7 +184,7 @@ union Joint {
 // workgroup's waves: the rows' outputs (part null), or the slot's share of them,
 // at part[row of all rows][HD] and ml[row], to be joined. RT 0: 8 rows or fewer
 // in one product; else RT tiles of 16.
-template <int HD, int KVT, int RT, class Masks>
+template <int HD, int KVT, int RT, bool CAP, class Masks>
 __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, const Walk& w, int slot, int slots, float* part,
                                           float2* ml, Joint<HD, RT>& sh, Masks masks) {
   constexpr bool PACK = RT == 0;
@@ -194,7 +194,6 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, kq = lane >> 4;
   const int b0 = slot * kW + wave, step = slots * kW;
-  const bool cap = a.softcap > 0.f;
 
   // the tile's q, 8 values a thread, requested ahead of the first block
   constexpr int kChunks = kRows * HD / 8, kTurns = (kChunks + kW * 64 - 1) / (kW * 64);
@@ -239,8 +238,8 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
       }
       amax = max_lanes<HD / 8>(amax);
       int e = 0;
-      const float c0 = cap ? a.scale : a.scale * kLog2e;
-      const float c1 = cap ? 0.f : __builtin_fmaf(a.scale, kLog2e, -c0) + a.scale * kLog2eLow;
+      const float c0 = CAP ? a.scale : a.scale * kLog2e;
+      const float c1 = CAP ? 0.f : __builtin_fmaf(a.scale, kLog2e, -c0) + a.scale * kLog2eLow;
       frexpf(amax * c0, &e);
       const int shift = min(max(14 - e, -100), 100);
       const float s0 = ldexpf(c0, shift), s1 = ldexpf(c1, shift);
@@ -314,29 +313,47 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
     blk.load_k(w, key, limit, n, kq);
     __builtin_amdgcn_sched_barrier(0);
 
-    v8h ph[NT], pl[PACK ? 1 : NT];
+    // the softmax of all tiles in straight code but for what happens seldom: a
+    // block that some row does not see in full, a maximum that grows past the lag
+    float vsc[KVT ? 8 : 1];
+    if constexpr (KVT == 1) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float vsc[KVT ? 8 : 1];
-      if constexpr (KVT == 1) {
+      for (int i = 0; i < 8; ++i) vsc[i] = blk.vs[i];
+    }
+    if constexpr (CAP) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) vsc[i] = blk.vs[i];
-      }
-      if (cap) {
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 8; ++i) sc[t][i] = span_cap(sc[t][i] * qscale[t], a);
-      }
-      masks.apply(at, end, kq, row[t], [&](int i) {
-        sc[t][i] = -INFINITY;
-        if constexpr (KVT == 1) vsc[i] = 0.f;
-      });
-      const float qs = cap ? kLog2e : qscale[t];
-      float bmax = sc[t][0];
+    }
+    uint32_t hidden[NT];   // int8: bit i, this lane's key i is not seen (its V scale may be infinite)
 #pragma unroll
-      for (int i = 1; i < 8; ++i) bmax = fmaxf(bmax, sc[t][i]);
-      bmax = max_pair(max_16(bmax)) * qs;
-      if (__any(bmax > m[t] + kLag)) {
-        const float mn = ceilf(fmaxf(m[t], bmax));
+    for (int t = 0; t < NT; ++t) hidden[t] = 0;
+    if (masks.some(at, end)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (masks.hides(at + 8 * kq + i, end, row[t])) {
+            sc[t][i] = -INFINITY;
+            hidden[t] |= 1u << i;
+          }
+    }
+    float qs[NT], bmax[NT];
+    bool grows = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      qs[t] = CAP ? kLog2e : qscale[t];
+      bmax[t] = sc[t][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) bmax[t] = fmaxf(bmax[t], sc[t][i]);
+      bmax[t] = max_pair(max_16(bmax[t])) * qs[t];
+      grows = grows || bmax[t] > m[t] + kLag;
+    }
+    if (__any(grows)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float mn = ceilf(bmax[t] > m[t] + kLag ? fmaxf(m[t], bmax[t]) : m[t]);
         const float corr = pow2(m[t] - (mn == -INFINITY ? 0.f : mn));
         l[t] *= corr;
         if (KVT == 0 && b != b0) {   // (nothing there yet)
@@ -345,44 +362,65 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
         }
         m[t] = mn;
       }
-      const float mo = m[t] == -INFINITY ? 0.f : m[t];
-      float pv[8];
+    }
+    float pv[NT][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) pv[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], qs, -mo));
-      l[t] += ((pv[0] + pv[4]) + (pv[1] + pv[5])) + ((pv[2] + pv[6]) + (pv[3] + pv[7]));
-      if constexpr (KVT == 1) {
-        float bx = 0.f;
+    for (int t = 0; t < NT; ++t) {
+      const float mo = m[t] == -INFINITY ? 0.f : m[t];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pv[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], qs[t], -mo));
+      l[t] += ((pv[t][0] + pv[t][4]) + (pv[t][1] + pv[t][5])) + ((pv[t][2] + pv[t][6]) + (pv[t][3] + pv[t][7]));
+    }
+    if constexpr (KVT == 1) {
+      float x[NT], bx[NT];
+      bool up = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        bx[t] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          pv[i] *= vsc[i];
-          bx = fmaxf(bx, pv[i]);
+          pv[t][i] *= hidden[t] >> i & 1 ? 0.f : vsc[i];
+          bx[t] = fmaxf(bx[t], pv[t][i]);
         }
-        bx = max_pair(max_16(bx));   // below 2^(e + 1)
-        const float x = m[t] + (float)max((int)(__float_as_uint(bx) >> 23) - 127, -100);
-        if (__any(bx > 0.f && x > ex[t] + kLagX)) {
-          const float en = bx > 0.f ? fmaxf(ex[t], x) : ex[t];
+        bx[t] = max_pair(max_16(bx[t]));   // below 2^(e + 1)
+        x[t] = m[t] + (float)max((int)(__float_as_uint(bx[t]) >> 23) - 127, -100);
+        up = up || (bx[t] > 0.f && x[t] > ex[t] + kLagX);
+      }
+      if (__any(up)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float en = bx[t] > 0.f && x[t] > ex[t] + kLagX ? x[t] : ex[t];
           const float corr = en == ex[t] ? 1.f : pow2(ex[t] - en);
 #pragma unroll
           for (int j = 0; j < DPL; ++j) o[t][j] *= corr;
           ex[t] = en;
         }
-        const int up = (int)fminf(kPExp + m[t] - ex[t], 126.f);   // (past 126 with every pv 0 only)
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int to = (int)fminf(kPExp + m[t] - ex[t], 126.f);   // (past 126 with every pv 0 only)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          pv[i] = ldexpf(pv[i], up);
-          asm("" : "+v"(pv[i]));   // rounded to fp32 before it is split
+          pv[t][i] = ldexpf(pv[t][i], to);
+          asm("" : "+v"(pv[t][i]));   // rounded to fp32 before it is split
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pv[i] *= kPScale;
       }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pv[t][i] *= kPScale;
+    }
+    v8h ph[NT], pl[PACK ? 1 : NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
       if constexpr (PACK) {
         v8h hi, lo;
-        split8(pv, hi, lo);
+        split8(pv[t], hi, lo);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ph[t][i] = n < 8 ? hi[i] : lo[i];
       } else {
-        split8(pv, ph[t], pl[t]);
+        split8(pv[t], ph[t], pl[t]);
       }
     }
 #pragma unroll
@@ -462,36 +500,32 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
 
 // Keys at or past the block's end are not there.
 struct TailMask {
-  template <class F>
-  __device__ __forceinline__ void apply(int key, int limit, int kq, int row, F hide) const {
-    if (key + kKeys > limit) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (key + 8 * kq + i >= limit) hide(i);
-    }
-  }
+  __device__ __forceinline__ bool some(int key, int limit) const { return key + kKeys > limit; }
+  __device__ __forceinline__ bool hides(int key, int limit, int row) const { return key >= limit; }
 };
 // Rows of several tokens: row r's token sees its own window alone.
 struct WindowMask {
   int gs, pos0, window, sinks, t0, t1;   // the tile's first and last token
-  template <class F>
-  __device__ __forceinline__ void apply(int key, int limit, int kq, int row, F hide) const {
-    if (key + kKeys <= limit && key + kKeys - 1 <= pos0 + t0 && (key > pos0 + t1 - window || key + kKeys <= sinks)) return;
-    const int lim = pos0 + min(row >> gs, t1), low = lim - window;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int j = key + 8 * kq + i;
-      if (j >= limit || j > lim || (j <= low && j >= sinks)) hide(i);
-    }
+  __device__ __forceinline__ bool some(int key, int limit) const {
+    return key + kKeys > limit || key + kKeys - 1 > pos0 + t0 || (key <= pos0 + t1 - window && key + kKeys > sinks);
+  }
+  __device__ __forceinline__ bool hides(int key, int limit, int row) const {
+    const int lim = pos0 + min(row >> gs, t1);
+    return key >= limit || key > lim || (key <= lim - window && key >= sinks);
   }
 };
 
-// Grid: n_kv_heads x slots.
-template <int HD, int KVT, int RT>
+// Grid: n_kv_heads x slots x tiles of rows.
+template <int HD, int KVT, int RT, bool CAP>
 __global__ void __launch_bounds__(kW * 64, simd_waves(HD)) k_span_window(const SpanArgs a, int slots) {
   __shared__ Joint<HD, RT> sh;
-  const int kvh = blockIdx.x % a.n_kv_heads, slot = blockIdx.x / a.n_kv_heads;
-  const int end = a.pos0 + a.n, rows = a.n * a.n_kv_heads << a.gs;
+  int i = blockIdx.x;
+  const int kvh = i % a.n_kv_heads;
+  i /= a.n_kv_heads;
+  const int slot = i % slots, tile = i / slots, rows = a.n * a.n_kv_heads << a.gs;
+  const int r0 = tile * tile_rows(RT);
+  const Rows r = {r0, min(r0 + tile_rows(RT), a.n << a.gs), kvh};
+  const int t0 = r.r0 >> a.gs, t1 = (r.r1 - 1) >> a.gs, end = a.pos0 + t1 + 1;   // its tokens
   Walk w;
   const size_t base = (size_t)kvh * a.max_seq * Block<HD, KVT>::kRowB;
   w.k = static_cast<const uint8_t*>(a.kc) + base;
@@ -499,22 +533,21 @@ __global__ void __launch_bounds__(kW * 64, simd_waves(HD)) k_span_window(const S
   w.ks = a.ks;
   w.vs = a.vs;
   w.to0 = min(a.sinks, end);
-  w.from1 = max(w.to0, a.pos0 + 1 - a.window);
+  w.from1 = max(w.to0, a.pos0 + t0 + 1 - a.window);
   w.to1 = end;
   w.nb0 = blocks_of(w.to0);
   w.nb = w.nb0 + blocks_of(w.to1 - w.from1);
-  const Rows r = {0, a.n << a.gs, kvh};
   float* part = slots > 1 ? slot_part<HD>(a, rows, slot) : nullptr;
   float2* ml = slot_ml<HD>(a, rows, slots, slot);
   if (a.n == 1)
-    span_tile<HD, KVT, RT>(a, r, w, slot, slots, part, ml, sh, TailMask{});
+    span_tile<HD, KVT, RT, CAP>(a, r, w, slot, slots, part, ml, sh, TailMask{});
   else
-    span_tile<HD, KVT, RT>(a, r, w, slot, slots, part, ml, sh, WindowMask{a.gs, a.pos0, a.window, a.sinks, 0, a.n - 1});
+    span_tile<HD, KVT, RT, CAP>(a, r, w, slot, slots, part, ml, sh, WindowMask{a.gs, a.pos0, a.window, a.sinks, t0, t1});
 }
 
 // Grid: n_kv_heads x np x tiles of rows over the prefix, then n_kv_heads x no x
 // sequences over their own caches; slots 0 .. np - 1 are the prefix's.
-template <int HD, int KVT, int RT>
+template <int HD, int KVT, int RT, bool CAP>
 __global__ void __launch_bounds__(kW * 64, simd_waves(HD)) k_span_shared(const SpanArgs a, int np, int no, int tiles) {
   __shared__ union {
     Joint<HD, RT> tile;
@@ -537,7 +570,7 @@ __global__ void __launch_bounds__(kW * 64, simd_waves(HD)) k_span_shared(const S
     w.nb = blocks_of(w.to1);
     const int r0 = tile * tile_rows(RT);
     const Rows r = {r0, min(r0 + tile_rows(RT), a.n << a.gs), kvh};
-    span_tile<HD, KVT, RT>(a, r, w, slot, np, slots > 1 ? slot_part<HD>(a, rows, slot) : nullptr,
+    span_tile<HD, KVT, RT, CAP>(a, r, w, slot, np, slots > 1 ? slot_part<HD>(a, rows, slot) : nullptr,
                               slot_ml<HD>(a, rows, slots, slot), sh.tile, TailMask{});
   } else {
     i -= np * tiles;
@@ -550,7 +583,7 @@ __global__ void __launch_bounds__(kW * 64, simd_waves(HD)) k_span_shared(const S
     w.to1 = own_length(a, t);
     w.nb = blocks_of(w.to1);
     const Rows r = {t << a.gs, t + 1 << a.gs, kvh};
-    span_tile<HD, KVT, 0>(a, r, w, slot, no, slots > 1 ? slot_part<HD>(a, rows, np + slot) : nullptr,
+    span_tile<HD, KVT, 0, CAP>(a, r, w, slot, no, slots > 1 ? slot_part<HD>(a, rows, np + slot) : nullptr,
                              slot_ml<HD>(a, rows, slots, np + slot), sh.own, TailMask{});
   }
 }
@@ -620,17 +653,21 @@ int rt_of(int hd, int rows) { return rows <= 8 ? 0 : rows <= 16 || hd == 256 ? 1
 
 // first, rest: the positions of the two spans that the window's rows see between them
 Plan plan_window(int hd, int group, int n_kv_heads, int n, int64_t first, int64_t rest, int n_cu) {
-  const int64_t rows = (int64_t)n * group, nb = (first + kKeys - 1) / kKeys + (rest + kKeys - 1) / kKeys;
+  const int64_t rows = (int64_t)n * group;
   Plan p = {rt_of(hd, (int)rows), 1, 1, 0};
-  if (rows > tile_rows(p.rt)) {
+  p.tiles = up(rows, tile_rows(p.rt));
+  // a tile's tokens see as many positions less than all of them
+  const int64_t apart = n - 1 - (tile_rows(p.rt) / group < n ? tile_rows(p.rt) / group : n);
+  const int64_t nb = (first + kKeys - 1) / kKeys + (rest - (apart > 0 ? apart : 0) + kKeys - 1) / kKeys;
+  if (rows > 32) {
     p.rt = -1;
-    flash_span_shape(hd, (int)rows, n_kv_heads, nb, n_cu, p.tiles, p.np);
+    flash_span_shape(hd, (int)rows, n_kv_heads, (first + kKeys - 1) / kKeys + (rest + kKeys - 1) / kKeys, n_cu, p.tiles, p.np);
     return p;
   }
   // A block per wave, up to two workgroups per compute unit; up to three blocks
   // per wave one workgroup does without the join (32 heads on 8, head_dim 128: 9
   // blocks 5.9 us, in three slots 7.6; 33 blocks 12.3 us, in nine slots 7.9).
-  const int64_t want = nb <= 3 * kW ? 1 : (nb + kW - 1) / kW, most = up(2 * n_cu, n_kv_heads);
+  const int64_t want = nb <= 3 * kW ? 1 : (nb + kW - 1) / kW, most = up(2 * n_cu, (int64_t)n_kv_heads * p.tiles);
   p.np = (int)(want < most ? want : most);
   return p;
 }
@@ -663,12 +700,18 @@ hipError_t launch_join(const SpanArgs& a, int slots, hipStream_t s) {
 template <int HD, int KVT, int RT>
 hipError_t launch_rt(const SpanArgs& a, const Plan& p, hipStream_t s) {
   const dim3 block(kW * 64);
-  const int64_t wgs = (int64_t)a.n_kv_heads * (a.own_len ? (int64_t)p.np * p.tiles + (int64_t)p.no * a.n : p.np);
+  const int64_t wgs = (int64_t)a.n_kv_heads * ((int64_t)p.np * p.tiles + (a.own_len ? (int64_t)p.no * a.n : 0));
   if (wgs > INT32_MAX) return hipErrorInvalidValue;
-  if (a.own_len)
-    hipLaunchKernelGGL((k_span_shared<HD, KVT, RT>), dim3((unsigned)wgs), block, 0, s, a, p.np, p.no, p.tiles);
+  const dim3 grid((unsigned)wgs);
+  const bool cap = a.softcap > 0.f;
+  if (a.own_len && cap)
+    hipLaunchKernelGGL((k_span_shared<HD, KVT, RT, true>), grid, block, 0, s, a, p.np, p.no, p.tiles);
+  else if (a.own_len)
+    hipLaunchKernelGGL((k_span_shared<HD, KVT, RT, false>), grid, block, 0, s, a, p.np, p.no, p.tiles);
+  else if (cap)
+    hipLaunchKernelGGL((k_span_window<HD, KVT, RT, true>), grid, block, 0, s, a, p.np);
   else
-    hipLaunchKernelGGL((k_span_window<HD, KVT, RT>), dim3((unsigned)wgs), block, 0, s, a, p.np);
+    hipLaunchKernelGGL((k_span_window<HD, KVT, RT, false>), grid, block, 0, s, a, p.np);
   return hipGetLastError();
 }
 
