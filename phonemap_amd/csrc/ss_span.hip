@@ -644,42 +644,64 @@ __global__ void __launch_bounds__(kJoinThreads) k_span_join(const SpanArgs a, in
 int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // How a call is cut: rt (tile_rows), tiles of rows, slots of the window or the
-// prefix (np) and of the own caches (no). A window's rt -1: more rows than a
-// decode step's, for ss_flash_span.hip.
+// prefix (np) and of the own caches (no). rt -1: a window's rows for the prompt
+// rows' kernel (ss_flash_span.hip).
 struct Plan {
   int rt, tiles, np, no;
 };
-int rt_of(int hd, int rows) { return rows <= 8 ? 0 : rows <= 16 || hd == 256 ? 1 : 2; }
+int rt_of(int hd, int64_t rows) { return rows <= 8 ? 0 : rows <= 16 || hd == 256 ? 1 : 2; }
+// workgroups that a device holds at once
+int64_t room(int hd, int n_cu) { return (int64_t)n_cu * simd_waves(hd); }
+
+// Blocks that a wave should walk when `rows` query rows of nb blocks are left to
+// slots: a block takes a wave some 0.35 us, and a slot's share costs a row 0.26 ns
+// to write and to join (head_dim 128), so nb / (4 each) slots are cheapest at each
+// = sqrt(nb rows hd / 128 * 1.9e-4). In us: 1 token, 33 blocks, 32 rows 7.9 with
+// one block each, 8.5 with two; 9 tokens, 131 blocks, 288 rows 17.1 and 15.6; 77
+// tokens, 34 blocks, 1232 rows at head_dim 256 31.3, two 26.6, four 20.4, eight 25.6.
+double blocks_each(int hd, int64_t nb, int64_t rows) { return sqrt((double)nb * (double)rows * hd / 128 * 1.9e-4); }
+int slots_of(int64_t nb, double each, int64_t most) {
+  if (each < 1.0) each = 1.0;
+  // up to three blocks per wave a single slot does without the join (9 blocks 5.9
+  // us, in three slots 7.6)
+  if (nb <= 3 * kW || most <= 1) return nb > 0 ? 1 : 0;
+  const int64_t want = (int64_t)ceil((double)nb / (kW * each));
+  return (int)(want < 1 ? 1 : want < most ? want : most);
+}
 
 // first, rest: the positions of the two spans that the window's rows see between them
 Plan plan_window(int hd, int group, int n_kv_heads, int n, int64_t first, int64_t rest, int n_cu) {
   const int64_t rows = (int64_t)n * group;
-  Plan p = {rt_of(hd, (int)rows), 1, 1, 0};
-  p.tiles = up(rows, tile_rows(p.rt));
+  Plan p = {rt_of(hd, rows), 1, 1, 0};
+  const int tile = tile_rows(p.rt), tokens = tile < rows ? (tile + group - 1) / group : n;
+  p.tiles = up(rows, tile);
   // a tile's tokens see as many positions less than all of them
-  const int64_t apart = n - 1 - (tile_rows(p.rt) / group < n ? tile_rows(p.rt) / group : n);
-  const int64_t nb = (first + kKeys - 1) / kKeys + (rest - (apart > 0 ? apart : 0) + kKeys - 1) / kKeys;
-  if (rows > 32) {
+  const int64_t nb = up(first, kKeys) + up(rest - (n - tokens) > 0 ? rest - (n - tokens) : 0, kKeys) + (p.tiles > 1);
+  // With many blocks per wave the prompt rows' kernel, whose waves share K and V,
+  // is ahead (512 tokens over 4096 positions, 32 heads on 8: 78 us, this one 82;
+  // 100 tokens 31 and 36; 32 tokens 21 and 19; 100 tokens over 300 positions 17 and 11).
+  if (p.tiles > 1 && nb * p.tiles * n_kv_heads > (int64_t)n_cu * 4 * 8) {
     p.rt = -1;
-    flash_span_shape(hd, (int)rows, n_kv_heads, (first + kKeys - 1) / kKeys + (rest + kKeys - 1) / kKeys, n_cu, p.tiles, p.np);
+    flash_span_shape(hd, (int)rows, n_kv_heads, up(first, kKeys) + up(rest, kKeys), n_cu, p.tiles, p.np);
     return p;
   }
-  // A block per wave, up to two workgroups per compute unit; up to three blocks
-  // per wave one workgroup does without the join (32 heads on 8, head_dim 128: 9
-  // blocks 5.9 us, in three slots 7.6; 33 blocks 12.3 us, in nine slots 7.9).
-  const int64_t want = nb <= 3 * kW ? 1 : (nb + kW - 1) / kW, most = up(2 * n_cu, (int64_t)n_kv_heads * p.tiles);
-  p.np = (int)(want < most ? want : most);
+  p.np = slots_of(nb, blocks_each(hd, nb, rows * n_kv_heads), room(hd, n_cu) / ((int64_t)n_kv_heads * p.tiles));
   return p;
 }
 Plan plan_shared(int hd, int group, int n_kv_heads, int n, int prefix, int own_max, int n_cu) {
-  const int rows = n * group, nbp = up(prefix, kKeys), nbo = up(own_max, kKeys);
+  const int64_t rows = (int64_t)n * group, nbp = up(prefix, kKeys), nbo = up(own_max, kKeys);
   Plan p;
   p.rt = prefix ? rt_of(hd, rows) : 0;
   p.tiles = prefix ? up(rows, tile_rows(p.rt)) : 0;
-  const int64_t all = ((int64_t)nbp * p.tiles + (int64_t)nbo * n) * n_kv_heads;
-  const int each = up(all, (int64_t)n_cu * 2 * kW);   // blocks per wave
-  p.np = up(nbp, (int64_t)kW * each);
-  p.no = up(nbo, (int64_t)kW * each);
+  // all workgroups at once, if that is not cheaper still with fewer slots
+  const double full = (double)(nbp * p.tiles + nbo * n) * n_kv_heads / (double)(room(hd, n_cu) * kW);
+  const double each = fmax(full, blocks_each(hd, nbp > nbo ? nbp : nbo, rows * n_kv_heads));
+  p.np = slots_of(nbp, each, INT32_MAX);
+  // More tiles than compute units: as many on each (64 sequences over 32000
+  // positions, 64 tiles: four slots 110 us, three 124, five 131, seven 117, eight 118).
+  const int64_t part = (int64_t)p.tiles * n_kv_heads;
+  if (part * p.np > n_cu && part <= n_cu) p.np = (int)(part * p.np / n_cu * n_cu / part);
+  p.no = slots_of(nbo, each, INT32_MAX);
   return p;
 }
 size_t plan_bytes(const Plan& p, int head_dim, int64_t rows) {
