@@ -215,8 +215,9 @@ int32_t ss_hip_sample_logits(ss_hip_ctx_t *ctx, const float *logits_dev, int32_t
  * (0: NULL will do), 16-byte aligned, its contents of no account before and
  * after. Calls that may run at the same time (two streams, two captured
  * graphs) need workspaces of their own; calls in one stream can share one.
- * Queries, outputs and caches are 16-byte aligned. The workspace functions
- * return 0 for a shape that the call refuses. */
+ * Queries, outputs and caches are 16-byte aligned; an output overlaps no
+ * input; a cache holds at most 2^30 positions. The workspace functions return 0
+ * for a shape that the call refuses. */
 
 /* Attention of the newest n_tokens of a sequence, at positions pos0 ..
  * pos0 + n_tokens - 1, each over a sliding window and the sequence's first
@@ -225,7 +226,8 @@ int32_t ss_hip_sample_logits(ss_hip_ctx_t *ctx, const float *logits_dev, int32_t
  * (n_tokens 1: a decode step), over either cache type (scales as
  * ss_hip_kv_append writes them); the cache already holds the tokens' own K
  * and V. softcap > 0 turns a score s into softcap * tanh(s / softcap) first
- * (Gemma 2); 0: none. Reads only positions that some token sees. */
+ * (Gemma 2; at least the least normal float); 0: none. Reads only positions
+ * that some token sees. A workspace serves every pos0. */
 size_t ss_hip_attention_window_workspace(ss_hip_ctx_t *ctx, int32_t n_heads, int32_t n_kv_heads,
                                          int32_t head_dim, int32_t n_tokens, int32_t window,
                                          int32_t n_sinks);

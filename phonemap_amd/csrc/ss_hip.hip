@@ -11,6 +11,7 @@
 #include "ss_hip.h"
 
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -608,7 +609,7 @@ int32_t span_setup(ss_hip_ctx_t* c, const char* what, ssk::SpanArgs& a, float* o
                    const void* vc, const float* ksc, const float* vsc, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                    int32_t n, float softcap, int32_t kv_type, bool used = true) {
   if (!out || !q || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || (kv_type != 0 && kv_type != 1) ||
-      (kv_type == 1 && used && (!ksc || !vsc)) || !(softcap >= 0.f) || isinf(softcap))
+      (kv_type == 1 && used && (!ksc || !vsc)) || !(softcap >= 0.f) || isinf(softcap) || (softcap > 0.f && softcap < FLT_MIN))
     return fail(kErrParams, "%s: bad argument", what);
   if (!ssk::attention_supported(head_dim, n_heads / n_kv_heads))
     return fail(kErrParams, "%s: head_dim %d / group %d not supported", what, head_dim, n_heads / n_kv_heads);
@@ -631,6 +632,9 @@ int32_t span_setup(ss_hip_ctx_t* c, const char* what, ssk::SpanArgs& a, float* o
   a.n_cu = c->n_cu;
   return 0;
 }
+
+// positions of a cache that the walks' 32-bit keys, some blocks past its end, count
+constexpr int32_t kMaxPositions = 1 << 30;
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
@@ -761,7 +765,8 @@ int32_t ss_hip_attention_window(ss_hip_ctx_t* c, float* out, const float* q, con
                                 int32_t head_dim, int32_t max_seq, int32_t pos0, int32_t n_tokens, int32_t window,
                                 int32_t n_sinks, float softcap, int32_t kv_type, void* ws, size_t ws_bytes,
                                 void* stream) {
-  if (!c || !kc || !vc || pos0 < 0 || n_tokens <= 0 || (int64_t)pos0 + n_tokens > max_seq || window <= 0 || n_sinks < 0)
+  if (!c || !kc || !vc || pos0 < 0 || n_tokens <= 0 || (int64_t)pos0 + n_tokens > max_seq || max_seq > kMaxPositions ||
+      window <= 0 || n_sinks < 0)
     return fail(kErrParams, "attention_window: bad argument (pos0 %d, %d tokens, max_seq %d, window %d, %d sinks)", pos0,
                 n_tokens, max_seq, window, n_sinks);
   ssk::SpanArgs a;
@@ -779,13 +784,15 @@ int32_t ss_hip_attention_window(ss_hip_ctx_t* c, float* out, const float* q, con
   a.part = static_cast<float*>(ws);
   DeviceScope on(c->device);
   HIP_TRY(on.status);
-  HIP_TRY(ssk::launch_span(head_dim, kv_type, a, pick(c, stream)));
+  HIP_TRY(ssk::launch_span(head_dim, kv_type, a, ws ? ws_bytes : 0, pick(c, stream)));
   return 0;
 }
 
 size_t ss_hip_attention_shared_workspace(ss_hip_ctx_t* c, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                          int32_t n_seqs, int32_t prefix_len, int32_t own_max) {
-  if (!c || !span_shape_ok(n_heads, n_kv_heads, head_dim, n_seqs) || prefix_len < 0 || own_max <= 0) return 0;
+  if (!c || !span_shape_ok(n_heads, n_kv_heads, head_dim, n_seqs) || prefix_len < 0 || prefix_len > kMaxPositions ||
+      own_max <= 0 || own_max > kMaxPositions)
+    return 0;
   return ssk::span_shared_workspace(head_dim, n_heads / n_kv_heads, n_kv_heads, n_seqs, prefix_len, own_max, c->n_cu);
 }
 
@@ -796,7 +803,7 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, con
                                 int32_t n_kv_heads, int32_t head_dim, float softcap, int32_t kv_type, void* ws,
                                 size_t ws_bytes, void* stream) {
   if (!c || !k_own || !v_own || !own_len || n_seqs <= 0 || own_max <= 0 || prefix_len < 0 || prefix_len > prefix_max ||
-      (prefix_len > 0 && (!k_prefix || !v_prefix)))
+      prefix_max > kMaxPositions || own_max > kMaxPositions || (prefix_len > 0 && (!k_prefix || !v_prefix)))
     return fail(kErrParams, "attention_shared: bad argument (%d sequences, prefix %d of %d, own_max %d)", n_seqs, prefix_len,
                 prefix_max, own_max);
   ssk::SpanArgs a;
@@ -821,7 +828,7 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, con
   a.part = static_cast<float*>(ws);
   DeviceScope on(c->device);
   HIP_TRY(on.status);
-  HIP_TRY(ssk::launch_span(head_dim, kv_type, a, pick(c, stream)));
+  HIP_TRY(ssk::launch_span(head_dim, kv_type, a, ws ? ws_bytes : 0, pick(c, stream)));
   return 0;
 }
 
@@ -2191,6 +2198,23 @@ uint64_t ss_hip_model_bytes(const ss_hip_model_t* m) { return m ? m->bytes : 0; 
 uint64_t ss_hip_model_host_bytes(const ss_hip_model_t* m) { return m ? m->host_bytes : 0; }
 
 int32_t ss_hip_model_launch(const ss_hip_model_t* m) { return m ? m->launch : -1; }
+
+// The bytes of its workspace that a window's call writes, from where it starts, on a
+// device of n_cu compute units; tests hold the workspace function to it. Not in the
+// public header.
+size_t ss_hip_attention_window_bytes(int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t pos0, int32_t n_tokens,
+                                     int32_t window, int32_t n_sinks, int32_t n_cu) {
+  if (!span_shape_ok(n_heads, n_kv_heads, head_dim, n_tokens)) return 0;
+  ssk::SpanArgs a = {};
+  a.n_kv_heads = n_kv_heads;
+  while (n_kv_heads << a.gs < n_heads) ++a.gs;
+  a.n = n_tokens;
+  a.pos0 = pos0;
+  a.window = window;
+  a.sinks = n_sinks;
+  a.n_cu = n_cu;
+  return ssk::span_bytes(head_dim, a);
+}
 
 // The shape a product of these sizes runs in on a device of n_cu compute units
 // (row tiles per workgroup); tests hold the rule to it. Not in the public header.

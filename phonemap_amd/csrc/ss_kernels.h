@@ -222,14 +222,16 @@ struct SpanArgs {
   float* part;               // workspace, as the functions below size it
   int n_cu;
 };
-hipError_t launch_span(int head_dim, int kv_type, const SpanArgs& a, hipStream_t s);
+// refuses a workspace of fewer than span_bytes
+hipError_t launch_span(int head_dim, int kv_type, const SpanArgs& a, size_t ws_bytes, hipStream_t s);
+size_t span_bytes(int head_dim, const SpanArgs& a);   // what this call writes of SpanArgs::part
 // The window's rows when they are more than a decode step's (ss_flash_span.hip),
 // their keys left to `slots` workgroups (more than one: shares for k_span_join).
 // The shape: tiles of rows and slots for `rows` query rows of a KV head over nb
 // blocks of 32 keys.
 void flash_span_shape(int head_dim, int rows, int n_kv_heads, int64_t nb, int n_cu, int& tiles, int& slots);
 hipError_t launch_flash_span(int head_dim, int kv_type, const SpanArgs& a, int slots, hipStream_t s);
-// bytes of SpanArgs::part; window and sinks at most max_seq
+// bytes of SpanArgs::part that serve every call of these sizes, wherever a window's rows start
 size_t span_window_workspace(int head_dim, int group, int n_kv_heads, int n, int window, int sinks, int n_cu);
 size_t span_shared_workspace(int head_dim, int group, int n_kv_heads, int n, int prefix, int own_max, int n_cu);
 // positions one attention workgroup covers in one round of loads

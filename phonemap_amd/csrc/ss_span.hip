@@ -669,6 +669,14 @@ int slots_of(int64_t nb, double each, int64_t most) {
   return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
+// The blocks of a window's call above which the prompt rows' kernel, whose waves
+// share K and V, takes it: many per wave (512 tokens over 4096 positions, 32 heads
+// on 8: 78 us, this file's 82; 100 tokens 31 and 36; 32 tokens 21 and 19; 100
+// tokens over 300 positions 17 and 11).
+int64_t span_blocks(int tiles, int n_kv_heads, int n_cu) {
+  return tiles > 1 ? (int64_t)n_cu * 4 * 8 / ((int64_t)tiles * n_kv_heads) : INT64_MAX;
+}
+
 // first, rest: the positions of the two spans that the window's rows see between them
 Plan plan_window(int hd, int group, int n_kv_heads, int n, int64_t first, int64_t rest, int n_cu) {
   const int64_t rows = (int64_t)n * group;
@@ -677,16 +685,26 @@ Plan plan_window(int hd, int group, int n_kv_heads, int n, int64_t first, int64_
   p.tiles = up(rows, tile);
   // a tile's tokens see as many positions less than all of them
   const int64_t nb = up(first, kKeys) + up(rest - (n - tokens) > 0 ? rest - (n - tokens) : 0, kKeys) + (p.tiles > 1);
-  // With many blocks per wave the prompt rows' kernel, whose waves share K and V,
-  // is ahead (512 tokens over 4096 positions, 32 heads on 8: 78 us, this one 82;
-  // 100 tokens 31 and 36; 32 tokens 21 and 19; 100 tokens over 300 positions 17 and 11).
-  if (p.tiles > 1 && nb * p.tiles * n_kv_heads > (int64_t)n_cu * 4 * 8) {
+  if (nb > span_blocks(p.tiles, n_kv_heads, n_cu)) {
     p.rt = -1;
     flash_span_shape(hd, (int)rows, n_kv_heads, up(first, kKeys) + up(rest, kKeys), n_cu, p.tiles, p.np);
     return p;
   }
   p.np = slots_of(nb, blocks_each(hd, nb, rows * n_kv_heads), room(hd, n_cu) / ((int64_t)n_kv_heads * p.tiles));
   return p;
+}
+
+// The most slots of any call with these rows, wherever it starts: with the whole
+// window behind it, and, where that is for the prompt rows' kernel, with the last
+// number of blocks that is not (the slots do not fall as the blocks grow, in either).
+int most_window_slots(int hd, int group, int n_kv_heads, int n, int64_t first, int64_t rest, int n_cu) {
+  const Plan p = plan_window(hd, group, n_kv_heads, n, first, rest, n_cu);
+  if (p.rt >= 0) return p.np;
+  const int64_t rows = (int64_t)n * group;
+  const int tiles = up(rows, tile_rows(rt_of(hd, rows)));
+  const int64_t nb = span_blocks(tiles, n_kv_heads, n_cu);
+  const int np = slots_of(nb, blocks_each(hd, nb, rows * n_kv_heads), room(hd, n_cu) / ((int64_t)n_kv_heads * tiles));
+  return np > p.np ? np : p.np;
 }
 Plan plan_shared(int hd, int group, int n_kv_heads, int n, int prefix, int own_max, int n_cu) {
   const int64_t rows = (int64_t)n * group, nbp = up(prefix, kKeys), nbo = up(own_max, kKeys);
@@ -704,8 +722,7 @@ Plan plan_shared(int hd, int group, int n_kv_heads, int n, int prefix, int own_m
   p.no = slots_of(nbo, each, INT32_MAX);
   return p;
 }
-size_t plan_bytes(const Plan& p, int head_dim, int64_t rows) {
-  const int slots = p.np + p.no;
+size_t slot_bytes(int slots, int head_dim, int64_t rows) {
   return slots < 2 ? 0 : (size_t)slots * rows * (head_dim + 2) * sizeof(float);
 }
 
@@ -759,24 +776,32 @@ hipError_t launch_hd(int kv_type, const SpanArgs& a, const Plan& p, hipStream_t 
 }  // namespace
 
 size_t span_window_workspace(int head_dim, int group, int n_kv_heads, int n, int window, int sinks, int n_cu) {
-  const Plan p = plan_window(head_dim, group, n_kv_heads, n, sinks, (int64_t)window + n - 1, n_cu);
-  return plan_bytes(p, head_dim, (int64_t)n * n_kv_heads * group);
+  return slot_bytes(most_window_slots(head_dim, group, n_kv_heads, n, sinks, (int64_t)window + n - 1, n_cu), head_dim,
+                    (int64_t)n * n_kv_heads * group);
 }
 size_t span_shared_workspace(int head_dim, int group, int n_kv_heads, int n, int prefix, int own_max, int n_cu) {
-  return plan_bytes(plan_shared(head_dim, group, n_kv_heads, n, prefix, own_max, n_cu), head_dim, (int64_t)n * n_kv_heads * group);
+  const Plan p = plan_shared(head_dim, group, n_kv_heads, n, prefix, own_max, n_cu);
+  return slot_bytes(p.np + p.no, head_dim, (int64_t)n * n_kv_heads * group);
 }
 
-hipError_t launch_span(int head_dim, int kv_type, const SpanArgs& a, hipStream_t s) {
+namespace {
+Plan plan_call(int head_dim, const SpanArgs& a) {
   const int group = 1 << a.gs;
-  if ((int64_t)a.n * a.n_kv_heads * group > INT32_MAX / 64) return hipErrorInvalidValue;
-  Plan p;
-  if (a.own_len) {
-    p = plan_shared(head_dim, group, a.n_kv_heads, a.n, a.prefix, a.own_max, a.n_cu);
-  } else {
-    const int end = a.pos0 + a.n, first = a.sinks < end ? a.sinks : end;
-    const int from = a.pos0 + 1 - a.window > first ? a.pos0 + 1 - a.window : first;
-    p = plan_window(head_dim, group, a.n_kv_heads, a.n, first, end - from, a.n_cu);
-  }
+  if (a.own_len) return plan_shared(head_dim, group, a.n_kv_heads, a.n, a.prefix, a.own_max, a.n_cu);
+  const int end = a.pos0 + a.n, first = a.sinks < end ? a.sinks : end;
+  const int from = a.pos0 + 1 - a.window > first ? a.pos0 + 1 - a.window : first;
+  return plan_window(head_dim, group, a.n_kv_heads, a.n, first, end - from, a.n_cu);
+}
+}  // namespace
+
+size_t span_bytes(int head_dim, const SpanArgs& a) {
+  const Plan p = plan_call(head_dim, a);
+  return slot_bytes(p.np + p.no, head_dim, (int64_t)a.n * a.n_kv_heads << a.gs);
+}
+
+hipError_t launch_span(int head_dim, int kv_type, const SpanArgs& a, size_t ws_bytes, hipStream_t s) {
+  if (((int64_t)a.n * a.n_kv_heads << a.gs) > INT32_MAX / 64 || span_bytes(head_dim, a) > ws_bytes) return hipErrorInvalidValue;
+  const Plan p = plan_call(head_dim, a);
   if (head_dim == 64) return launch_hd<64>(kv_type, a, p, s);
   if (head_dim == 128) return launch_hd<128>(kv_type, a, p, s);
   if (head_dim == 256) return launch_hd<256>(kv_type, a, p, s);

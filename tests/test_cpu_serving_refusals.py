@@ -91,9 +91,32 @@ def test_workspaces_of_refused_shapes():
 
 
 def test_workspaces_cover_every_position():
-    """The window's workspace goes by the window alone: no position asks for more."""
+    """The window's workspace goes by the window alone: no position asks for more.
+    (With the window behind them 200 tokens of 32 heads on 4, head_dim 64, are the
+    prompt rows' kernel's, in one piece; at position 600 they are two slots.)"""
     L, ctx = pm.lib(), _context()
     x = C.addressof(ctx)
+    assert L.ss_hip_attention_window_bytes(32, 4, 64, 600, 200, 1900, 4, 256) > 0
+    for heads, kv_heads in ((32, 4), (32, 8), (8, 1), (8, 8), (1, 1), (64, 8)):
+        for hd in (64, 128, 256):
+            for n in (1, 2, 3, 9, 17, 33, 40, 64, 100, 150, 200, 257, 400, 700, 1000, 3000):
+                for w, sinks in ((1, 0), (100, 4), (1900, 4), (5000, 0), (300, 900), (20000, 0), (2 ** 30, 0), (2 ** 31 - 1, 2 ** 31 - 1)):
+                    have = L.ss_hip_attention_window_workspace(x, heads, kv_heads, hd, n, w, sinks)
+                    for pos0 in (0, 1, 31, 64, 150, 300, 600, 777, 1500, 2500, 6000, 19999, 50000, 10 ** 6):
+                        end = pos0 + n + 3
+                        need = L.ss_hip_attention_window_bytes(heads, kv_heads, hd, pos0, n, min(w, end), min(sinks, end), 256)
+                        assert need <= have, (heads, kv_heads, hd, n, w, sinks, pos0)
     for n in (1, 3, 40):
         sizes = [L.ss_hip_attention_window_workspace(x, 32, 8, 128, n, w, 4) for w in (1, 10, 100, 1000, 5000, 20000, 2 ** 31 - 1)]
         assert sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("bad", [dict(max_seq=2 ** 30 + 1), dict(max_seq=2 ** 31 - 1), dict(cap=1e-40)], ids=str)
+def test_window_limits(bad):
+    _refused("ss_hip_attention_window", WINDOW, **bad)
+
+
+@pytest.mark.parametrize("bad", [dict(prefix_max=2 ** 30 + 1), dict(prefix_max=2 ** 31 - 1, prefix=2 ** 31 - 1),
+                                 dict(own_max=2 ** 30 + 1), dict(own_max=2 ** 31 - 1), dict(cap=1e-40)], ids=str)
+def test_shared_limits(bad):
+    _refused("ss_hip_attention_shared", SHARED, **bad)
