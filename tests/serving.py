@@ -10,6 +10,8 @@ relative error; q and the weights held to 2^-22 and the exponential's 2^-22 add
 11 bits gives 1e-5 to 2e-4 of a row, one key left out or taken twice 1e-4 and
 more at these lengths.
 """
+import ctypes as C
+
 import numpy as np
 
 TOL = 4e-6
@@ -195,3 +197,44 @@ def sample_call(hip, x, T, top_k, top_p, min_p, u, ld=None, stream=None):
     got = c.result()
     c.free()
     return got
+
+
+# ---- streams and graphs --------------------------------------------------------
+class Stream:
+    """A HIP stream, and captures of calls made on it; the runtime is the library's."""
+
+    def __init__(self, hip):
+        self.L, self.s = hip.L, C.c_void_p()
+        self.made = []
+        self.ok(self.L.hipStreamCreate(C.byref(self.s)))
+
+    @staticmethod
+    def ok(rc):
+        assert rc == 0, rc
+
+    @property
+    def ptr(self):
+        return self.s.value
+
+    def wait(self):
+        self.ok(self.L.hipStreamSynchronize(self.s))
+
+    def capture(self, calls):
+        """Records what calls() launches; returns what launches the graph."""
+        graph, run = C.c_void_p(), C.c_void_p()
+        self.ok(self.L.hipStreamBeginCapture(self.s, 1))   # hipStreamCaptureModeThreadLocal
+        try:
+            calls()
+        finally:
+            rc = self.L.hipStreamEndCapture(self.s, C.byref(graph))
+        self.ok(rc)
+        self.ok(self.L.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)))
+        self.ok(self.L.hipGraphDestroy(graph))
+        self.made.append(run)
+        return lambda: self.ok(self.L.hipGraphLaunch(run, self.s))
+
+    def free(self):
+        self.wait()
+        for run in self.made:
+            self.ok(self.L.hipGraphExecDestroy(run))
+        self.ok(self.L.hipStreamDestroy(self.s))
