@@ -18,8 +18,8 @@
 // O^T = V^T P^T wants of it as B. There lane (n, kq) supplies V^T[n][keys 8kq ..
 // 8kq + 7]: it loads its DPL = HD / 16 dimensions DPL n .. of each of these 8
 // keys (a load covers whole rows), and a v_perm per two values turns them
-// round; tile j of DPL is then dimension DPL m + j. K, or V, of the next block is
-// requested as soon as the current one's is used up.
+// round; tile j of DPL is then dimension DPL m + j. K of the next block is
+// requested as soon as the current one's is used up, V during the next scores.
 //
 // Precision is that of the prompt rows' kernel (ss_flash.h): K and V exact, q
 // and the weights as two fp16 parts, whole-number maxima in base 2, fp32 sums.
@@ -66,6 +66,26 @@ __device__ __forceinline__ float max_lanes(float v) {
   return v;
 }
 
+// hi + lo = v as split8 of ss_mfma.h does, less: -1
+__device__ __forceinline__ void split8(const float* v, v8h& hi, v8h& lo, float less) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) hi[i] = (_Float16)v[i];
+  v4u h = __builtin_bit_cast(v4u, hi);
+  asm("" : "+v"(h));   // (pairs, not converted a second time one by one)
+  hi = __builtin_bit_cast(v8h, h);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lo[i] = (_Float16)__builtin_fmaf((float)hi[i], less, v[i]);
+}
+
+// f(0), .., f(N - 1), of constants
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void each(const F& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<N, I + 1>(f);
+  }
+}
+
 // The tile's rows: row r is query head g of token or sequence t, t * G + g = r0 + r < r1.
 struct Rows {
   int r0, r1, kvh;
@@ -96,12 +116,14 @@ struct Block {
         k[t][c] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, at + 4 * t * kRowB + 64 * c, 0, 0));
     if constexpr (KVT == 1) scales(w.ks, key, live, kq, ks);
   }
+  // this lane's keys 8kq + FROM .. 8kq + TO - 1, and with the first the scales of all 8
+  template <int FROM, int TO>
   __device__ __forceinline__ void load_v(const Walk& w, int key, int limit, int n, int kq) {
     const int live = min(limit - key, kKeys);
     const auto r = view(w.v, (size_t)key * kRowB, live * kRowB);
     const int at = 8 * kq * kRowB + 4 * kVWords * n;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = FROM; i < TO; ++i) {
       if constexpr (kVWords == 1) {
         v[i][0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, at + i * kRowB, 0, 0);
       } else if constexpr (kVWords == 2) {
@@ -117,7 +139,7 @@ struct Block {
         }
       }
     }
-    if constexpr (KVT == 1) scales(w.vs, key, live, kq, vs);
+    if constexpr (KVT == 1 && FROM == 0) scales(w.vs, key, live, kq, vs);
   }
   static __device__ __forceinline__ void scales(const float* p, int key, int live, int kq, float (&s)[KVT ? 8 : 1]) {
     const auto r = view(p, (size_t)key * 4, live * 4);
@@ -220,7 +242,7 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
   };
   next(b0);
   blk.load_k(w, key, limit, n, kq);
-  blk.load_v(w, key, limit, n, kq);
+  blk.template load_v<0, 8>(w, key, limit, n, kq);
   __builtin_amdgcn_sched_barrier(0);
 
   // q times the softmax's scale and log2 e, a row's largest magnitude brought to
@@ -284,29 +306,41 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
     for (int j = 0; j < DPL; ++j) o[t][j] = v4f{};
   }
 
-#pragma unroll 1
-  for (int b = b0; b < w.nb; b += step) {
+  float less = -1.f;   // (in a register: what is left of a value is one mixed fma)
+  asm("" : "+s"(less));
+  // Block b. Its V is requested between its scores' products, the first one's
+  // ahead of them; the next one's K behind them. (Both at once, when their
+  // registers are free: 37 sequences, int8, 24.8 us instead of 24.3; 24 sequences
+  // over 8000 positions 24.8 and 24.3. K between the softmax's steps too: 64 over
+  // 32000 114 instead of 111.)
+  auto block = [&](int b, auto first) {
+    constexpr bool FIRST = decltype(first)::value;
     // the scores of keys key + 8kq + 0 .. 7
+    // (the chains of products in turn: one waits for its own last)
     float sc[NT][8];
+    v4f d[NT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      v4f d[2];
+    for (int t = 0; t < NT; ++t) d[t][0] = d[t][1] = v4f{};
+    constexpr int kGroups = (PACK ? 1 : 2) * NC * 2;   // of NT products
+    auto group = [&](auto gi) {
+      constexpr int i = decltype(gi)::value, c = i / 2 % NC, u = i % 2;
+      constexpr bool low = !PACK && i < NC * 2;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        d[u] = v4f{};
-        if constexpr (!PACK) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) d[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(blk.k_slice(u, c), ql[t][c], d[u], 0, 0, 0);
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) d[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(blk.k_slice(u, c), qh[t][c], d[u], 0, 0, 0);
+      for (int t = 0; t < NT; ++t)
+        d[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(blk.k_slice(u, c), low ? ql[PACK ? 0 : t][PACK ? 0 : c] : qh[t][c], d[t][u], 0, 0, 0);
+      if constexpr (!FIRST && (i + 1) * 8 / kGroups > i * 8 / kGroups) {
+        blk.template load_v<i * 8 / kGroups, (i + 1) * 8 / kGroups>(w, key, limit, n, kq);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    };
+    each<kGroups>(group);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        sc[t][i] = PACK ? d[i / 4][i % 4] + swap_8(d[i / 4][i % 4]) : d[i / 4][i % 4];
+        sc[t][i] = PACK ? d[t][i / 4][i % 4] + swap_8(d[t][i / 4][i % 4]) : d[t][i / 4][i % 4];
         if constexpr (KVT == 1) sc[t][i] *= blk.ks[i];
       }
-    }
     const int at = key, end = limit;
     __builtin_amdgcn_sched_barrier(0);
     next(b + step);
@@ -347,16 +381,17 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
       bmax[t] = sc[t][0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) bmax[t] = fmaxf(bmax[t], sc[t][i]);
-      bmax[t] = max_pair(max_16(bmax[t])) * qs[t];
+      bmax[t] *= qs[t];
       grows = grows || bmax[t] > m[t] + kLag;
     }
-    if (__any(grows)) {
+    if (__any(grows)) {   // (the row's other lanes are asked only now)
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        bmax[t] = max_pair(max_16(bmax[t]));
         const float mn = ceilf(bmax[t] > m[t] + kLag ? fmaxf(m[t], bmax[t]) : m[t]);
         const float corr = pow2(m[t] - (mn == -INFINITY ? 0.f : mn));
         l[t] *= corr;
-        if (KVT == 0 && b != b0) {   // (nothing there yet)
+        if (KVT == 0 && !FIRST) {   // (nothing there yet)
 #pragma unroll
           for (int j = 0; j < DPL; ++j) o[t][j] *= corr;
         }
@@ -366,14 +401,16 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
     float pv[NT][8];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const float mo = m[t] == -INFINITY ? 0.f : m[t];
+      // fp16: times 2^12, for the lower part's range (int8: below, by its exponent)
+      const float mo = (m[t] == -INFINITY ? 0.f : m[t]) - (KVT == 0 ? kPExp : 0.f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) pv[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], qs[t], -mo));
       l[t] += ((pv[t][0] + pv[t][4]) + (pv[t][1] + pv[t][5])) + ((pv[t][2] + pv[t][6]) + (pv[t][3] + pv[t][7]));
     }
     if constexpr (KVT == 1) {
-      float x[NT], bx[NT];
+      float bx[NT];
       bool up = false;
+      auto exponent = [](float b, float mt) { return mt + (float)max((int)(__float_as_uint(b) >> 23) - 127, -100); };
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         bx[t] = 0.f;
@@ -382,14 +419,14 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
           pv[t][i] *= hidden[t] >> i & 1 ? 0.f : vsc[i];
           bx[t] = fmaxf(bx[t], pv[t][i]);
         }
-        bx[t] = max_pair(max_16(bx[t]));   // below 2^(e + 1)
-        x[t] = m[t] + (float)max((int)(__float_as_uint(bx[t]) >> 23) - 127, -100);
-        up = up || (bx[t] > 0.f && x[t] > ex[t] + kLagX);
+        up = up || (bx[t] > 0.f && exponent(bx[t], m[t]) > ex[t] + kLagX);
       }
       if (__any(up)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const float en = bx[t] > 0.f && x[t] > ex[t] + kLagX ? x[t] : ex[t];
+          bx[t] = max_pair(max_16(bx[t]));   // below 2^(e + 1)
+          const float x = exponent(bx[t], m[t]);
+          const float en = bx[t] > 0.f && x > ex[t] + kLagX ? x : ex[t];
           const float corr = en == ex[t] ? 1.f : pow2(ex[t] - en);
 #pragma unroll
           for (int j = 0; j < DPL; ++j) o[t][j] *= corr;
@@ -405,42 +442,38 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
           asm("" : "+v"(pv[t][i]));   // rounded to fp32 before it is split
         }
       }
-    } else {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pv[t][i] *= kPScale;
     }
     v8h ph[NT], pl[PACK ? 1 : NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if constexpr (PACK) {
         v8h hi, lo;
-        split8(pv[t], hi, lo);
+        split8(pv[t], hi, lo, less);
 #pragma unroll
         for (int i = 0; i < 8; ++i) ph[t][i] = n < 8 ? hi[i] : lo[i];
       } else {
-        split8(pv[t], ph[t], pl[t]);
+        split8(pv[t], ph[t], pl[t], less);
       }
     }
 #pragma unroll
     for (int j = 0; j < DPL; ++j) {
       const v8h vt = blk.v_tile(j);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      for (int t = 0; t < NT; ++t)
         if constexpr (!PACK) o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, pl[t], o[t][j], 0, 0, 0);
-        o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, ph[t], o[t][j], 0, 0, 0);
-      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, ph[t], o[t][j], 0, 0, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
-    blk.load_v(w, key, limit, n, kq);
-    __builtin_amdgcn_sched_barrier(0);
-  }
+  };
+  if (b0 < w.nb) block(b0, std::true_type{});
+#pragma unroll 1
+  for (int b = b0 + step; b < w.nb; b += step) block(b, std::false_type{});
 
   // the waves' rows -> one
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    l[t] = sum_pair(sum_16(l[t]));
+    l[t] = sum_pair(sum_16(l[t])) * (KVT == 0 ? 1 / kPScale : 1.f);
     if constexpr (PACK) {
 #pragma unroll
       for (int j = 0; j < DPL; ++j)
