@@ -181,10 +181,12 @@ __device__ __forceinline__ void add_u64(uint64_t* p, uint64_t v) {
 
 // Selection by the bits of the keys, kDigit at a time: the largest key at which
 // the sum of val(i) over the entries i < n with that key or a greater one reaches
-// target, 0 when all together do not. hist: 2^kDigit words, red: NT / 64 + 2.
+// target, or a smaller one that parts the entries alike, 0 when all together do
+// not. one: what one entry's val is at most, and less than two entries' (0: not
+// known). hist: 2^kDigit words, red: NT / 64 + 3.
 constexpr int kDigit = 10, kDigits = 1 << kDigit;
 template <int NT, class Key, class Val>
-__device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_t* red, Key key, Val val) {
+__device__ uint32_t key_reaching(int n, uint64_t target, uint64_t one, uint64_t* hist, uint64_t* red, Key key, Val val) {
   constexpr int kEach = kDigits / NT;   // digits of a thread, the highest ones in thread 0
   static_assert(kEach * NT == kDigits, "whole");
   // the bits that all keys share
@@ -220,6 +222,7 @@ __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_
       if (before < target && before + h[c] >= target) {
         found[0] = kDigits - 1 - (kEach * (int)threadIdx.x + c);
         found[1] = before;
+        found[2] = h[c];
       }
       before += h[c];
     }
@@ -228,7 +231,9 @@ __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t* hist, uint64_
     prefix |= (uint32_t)found[0] << shift;
     mask |= digit << shift;
     above = found[1];
+    const bool alone = found[2] <= one;
     __syncthreads();
+    if (alone) break;   // (its key's low bits part it from nothing)
   } while (shift > 0);
   return prefix;
 }
@@ -454,8 +459,10 @@ __device__ uint32_t least_of(const Edge& e, const Keep& keep, const float* v, in
   }
   auto key = [&](int i) { return order(v[i]); };
   uint32_t k = 0;
-  if (e.need_k) k = key_reaching<NT>(n, e.need_k, digits, red, key, [](int) { return 1ull; });
-  if (e.need_p) k = max(k, key_reaching<NT>(n, e.need_p, digits, red, key, [&](int i) { return keep.scale.units(v[i], bin); }));
+  // (weights are e^-1/8 .. e^1/8 times 2^44, and a little)
+  constexpr uint64_t kOneWeight = 3ull << 43;
+  if (e.need_k) k = key_reaching<NT>(n, e.need_k, 1, digits, red, key, [](int) { return 1ull; });
+  if (e.need_p) k = max(k, key_reaching<NT>(n, e.need_p, kOneWeight, digits, red, key, [&](int i) { return keep.scale.units(v[i], bin); }));
   return k;
 }
 
@@ -466,12 +473,12 @@ __device__ int slow(const SampleRowsArgs& a, const float* x, float mx, float u, 
   auto key = [&](int i) { return order(x[i]); };
   auto weight = [&](int i) { return (uint64_t)(exp(gap(x[i], mx) / a.temperature) * kUnit + 0.5); };
   uint32_t least = 0;
-  if (a.top_k) least = key_reaching<NT>(V, (uint64_t)a.top_k, hist, red, key, [](int) { return 1ull; });
+  if (a.top_k) least = key_reaching<NT>(V, (uint64_t)a.top_k, 1, hist, red, key, [](int) { return 1ull; });
   if (a.top_p < 1.0) {
     uint64_t s = 0;
     for (int i = tid; i < V; i += NT) s += weight(i);
     const double goal = ceil(a.top_p * (double)group_sum<NT>(s, red));
-    least = max(least, key_reaching<NT>(V, (uint64_t)fmax(goal, 1.0), hist, red, key, weight));
+    least = max(least, key_reaching<NT>(V, (uint64_t)fmax(goal, 1.0), 0, hist, red, key, weight));
   }
   auto kept = [&](int i) { return key(i) >= least && gap(x[i], mx) >= a.min_gap ? weight(i) : 0; };
   // contiguous pieces: the thread in whose piece the running sum passes the draw
@@ -535,7 +542,7 @@ __global__ void __launch_bounds__(kOneThreads) k_one(const SampleRowsArgs a) {
   } sh;
   __shared__ Bins bins;
   __shared__ double fall[kBins], part[Row::kRounds * NT / 64];
-  __shared__ uint64_t red[NT / 64 + 2], digits[kDigits];
+  __shared__ uint64_t red[NT / 64 + 3], digits[kDigits];
   __shared__ uint32_t least;
   __shared__ int n;
   __shared__ Edge edge;
@@ -613,7 +620,7 @@ __host__ __device__ inline RowWork row_work(void* work, int row, int tiles, size
 __global__ void __launch_bounds__(kTileThreads) k_tiles(const SampleRowsArgs a) {
   constexpr int NT = kTileThreads, E = kTileEach;
   __shared__ Histogram<NT> h;
-  __shared__ uint64_t red[NT / 64 + 2];
+  __shared__ uint64_t red[NT / 64 + 3];
   const int tid = threadIdx.x, tile = blockIdx.x, row = blockIdx.y;
   const RowWork w = row_work(a.work, row, gridDim.x, nullptr);
   Chunk<NT, E> c;
@@ -648,7 +655,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   __shared__ int at[kList];
   __shared__ Bins bins;
   __shared__ double fall[kBins], kept[kMaxTiles], part[Tile::kRounds * kWaves];
-  __shared__ uint64_t red[kWaves + 2], digits[kDigits], edge_kept[kMaxTiles];
+  __shared__ uint64_t red[kWaves + 3], digits[kDigits], edge_kept[kMaxTiles];
   __shared__ uint32_t tops[kMaxTiles], least;
   __shared__ int n;
   __shared__ uint32_t base, done;
@@ -708,12 +715,17 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
   }
   if (filtered(a)) {
 #pragma unroll
-    for (int k = 0; k < kMost; ++k)
+    for (int h = 0; h < 2; ++h) {
+      uint64_t ws = 0;
+      uint32_t cs = 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (weight[k][h]) add_u64(&bins.weight[lane + 64 * h], weight[k][h]);
-        if (count[k][h]) atomicAdd(&bins.count[lane + 64 * h], count[k][h]);
+      for (int k = 0; k < kMost; ++k) {
+        ws += weight[k][h];
+        cs += count[k][h];
       }
+      if (ws) add_u64(&bins.weight[lane + 64 * h], ws);
+      if (cs) atomicAdd(&bins.count[lane + 64 * h], cs);
+    }
   }
   __syncthreads();
   if (tid < kWave) {
@@ -764,7 +776,7 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
 #pragma unroll
       for (int k = 0; k < kRounds; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) hit |= scale.bin(d[k].x[j]) == bin ? 1u << (4 * k + j) : 0u;
+        for (int j = 0; j < 4; ++j) hit |= floorf(d[k].x[j] * scale.per) == bin ? 1u << (4 * k + j) : 0u;   // (NaN: no)
       if (!__any(hit)) return;
       const uint64_t mine = __popc(hit), upto = wave_upto(mine);
       int p = 0;
