@@ -2,12 +2,16 @@
 device: the checks read the context's fields alone, so a block of zeros stands
 in for one. Every call here is refused."""
 import ctypes as C
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
 
 import phonemap_amd as pm
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CTX = (C.c_uint8 * 4096)()
 P = 1 << 20   # an aligned address; nothing is read there
 
@@ -120,3 +124,15 @@ def test_window_limits(bad):
                                  dict(own_max=2 ** 30 + 1), dict(own_max=2 ** 31 - 1), dict(cap=1e-40)], ids=str)
 def test_shared_limits(bad):
     _refused("ss_hip_attention_shared", SHARED, **bad)
+
+
+def test_header(tmp_path):
+    """ss_hip.h brings the serving calls with it, either header can come first, and each declared call is exported."""
+    text = open(os.path.join(ROOT, "include", "ss_hip_serving.h")).read()
+    names = set(re.findall(r"^(?:size_t|int32_t) (ss_hip_\w+)\(", text, flags=re.M))
+    assert names == {"ss_hip_%s%s" % (n, w) for n in ("attention_window", "attention_shared", "sample_rows") for w in ("", "_workspace")}
+    assert all(hasattr(pm.lib(), n) for n in names)
+    for first in ("ss_hip.h", "ss_hip_serving.h"):
+        src = tmp_path / "a.c"
+        src.write_text('#include "%s"\nvoid *calls[] = {%s};\n' % (first, ", ".join("(void *)" + n for n in sorted(names))))
+        subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(ROOT, "include"), str(src)], check=True)
