@@ -130,18 +130,22 @@ __device__ __forceinline__ void span_row(const SpanArgs& a, const float* q, floa
 constexpr int kKeys = 32;   // keys per block
 __device__ __forceinline__ int blocks_of(int n) { return (n + kKeys - 1) / kKeys; }
 
-// What a tile of rows walks: blocks of positions [0, to0), then of [from1, to1), of one KV head's K and V.
-struct Walk {
+// one KV head's K and V
+struct Base {
   const uint8_t* k;
   const uint8_t* v;
   const float* ks;
   const float* vs;
+};
+// What a tile of rows walks: blocks of positions [0, to0), then of [from1, to1).
+struct Walk : Base {
   int to0, from1, to1;
   int nb0, nb;   // blocks of the first span, of both
   __device__ __forceinline__ void block(int b, int& key, int& limit) const {
     key = b < nb0 ? kKeys * b : from1 + kKeys * (b - nb0);
     limit = b < nb0 ? to0 : to1;
   }
+  __device__ __forceinline__ Base base(int) const { return *this; }
 };
 
 // among all rows [n][n_heads]

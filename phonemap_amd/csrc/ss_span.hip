@@ -7,7 +7,8 @@
 // the waves of each in turn, so every wave has its own softmax; a workgroup
 // joins its waves through LDS, and k_span_join the slots. The sequences' rows
 // over their own caches (8 rows or fewer that share K and V) and tiles of all
-// sequences' rows over the prefix are workgroups of the same launch.
+// sequences' rows over the prefix are workgroups of the same launch; where both
+// caches are short a sequence's rows go through both in one workgroup.
 //
 // No LDS in the loop: K and V come from memory straight into the operands of
 // v_mfma_f32_16x16x32_f16 (lane l = (n, kq) = (l % 16, l / 16) supplies
@@ -105,7 +106,7 @@ struct Block {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(static_cast<const uint8_t*>(p) + from), (short)0, bytes,
                                              kBufferFlags);
   }
-  __device__ __forceinline__ void load_k(const Walk& w, int key, int limit, int n, int kq) {
+  __device__ __forceinline__ void load_k(const Base& w, int key, int limit, int n, int kq) {
     const int live = min(limit - key, kKeys);
     const auto r = view(w.k, (size_t)key * kRowB, live * kRowB);
     const int at = (8 * (n >> 2) + (n & 3)) * kRowB + 16 * kq;
@@ -118,7 +119,7 @@ struct Block {
   }
   // this lane's keys 8kq + FROM .. 8kq + TO - 1, and with the first the scales of all 8
   template <int FROM, int TO>
-  __device__ __forceinline__ void load_v(const Walk& w, int key, int limit, int n, int kq) {
+  __device__ __forceinline__ void load_v(const Base& w, int key, int limit, int n, int kq) {
     const int live = min(limit - key, kKeys);
     const auto r = view(w.v, (size_t)key * kRowB, live * kRowB);
     const int at = 8 * kq * kRowB + 4 * kVWords * n;
@@ -183,13 +184,13 @@ __device__ __forceinline__ int slice_dim(int c, int kq) {
 }
 
 __host__ __device__ constexpr int tile_rows(int rt) { return rt == 0 ? 8 : 16 * rt; }
-constexpr int kW = 4;   // waves of a workgroup
+constexpr int kW = 4, kWide = 8;   // waves of a workgroup, of k_span_each's
 // and at most that many per SIMD, by their registers
 __host__ __device__ constexpr int simd_waves(int hd) { return hd < 256 ? 2 : 1; }
 
 // A workgroup's LDS: first q, its parts as rows (n and rows + n) in the order of
 // the products' operand; then the waves' results.
-template <int HD, int RT>
+template <int HD, int RT, int W = kW>
 union Joint {
   static constexpr int kRows = tile_rows(RT);
   struct {
@@ -197,8 +198,8 @@ union Joint {
     float scale[kRows];
   } q;
   struct {
-    float o[kW][kRows][HD + 4];
-    float m[kW][kRows], l[kW][kRows], e[kW][kRows];
+    float o[W][kRows][HD + 4];
+    float m[W][kRows], l[W][kRows], e[W][kRows];
   } r;
 };
 
@@ -206,24 +207,24 @@ union Joint {
 // workgroup's waves: the rows' outputs (part null), or the slot's share of them,
 // at part[row of all rows][HD] and ml[row], to be joined. RT 0: 8 rows or fewer
 // in one product; else RT tiles of 16.
-template <int HD, int KVT, int RT, bool CAP, class Masks>
-__device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, const Walk& w, int slot, int slots, float* part,
-                                          float2* ml, Joint<HD, RT>& sh, Masks masks) {
+template <int HD, int KVT, int RT, bool CAP, int W = kW, class Walks, class Masks>
+__device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, const Walks& w, int slot, int slots, float* part,
+                                          float2* ml, Joint<HD, RT, W>& sh, Masks masks) {
   constexpr bool PACK = RT == 0;
   constexpr int kRows = tile_rows(RT), NT = PACK ? 1 : RT, NC = HD / 32, DPL = HD / 16;
   using Blk = Block<HD, KVT>;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, kq = lane >> 4;
-  const int b0 = slot * kW + wave, step = slots * kW;
+  const int b0 = slot * W + wave, step = slots * W;
 
   // the tile's q, 8 values a thread, requested ahead of the first block
-  constexpr int kChunks = kRows * HD / 8, kTurns = (kChunks + kW * 64 - 1) / (kW * 64);
+  constexpr int kChunks = kRows * HD / 8, kTurns = (kChunks + W * 64 - 1) / (W * 64);
   static_assert(kChunks % 64 == 0, "whole waves");
   float qv[kTurns][8];
 #pragma unroll
   for (int u = 0; u < kTurns; ++u) {
-    const int i = tid + u * kW * 64, row = rows.r0 + i / (HD / 8);
+    const int i = tid + u * W * 64, row = rows.r0 + i / (HD / 8);
     if (i < kChunks) {
       const float* qp = a.q + row_head(a, rows.kvh, min(row, rows.r1 - 1)) * HD + i % (HD / 8) * 8;
       const float4 x0 = *reinterpret_cast<const float4*>(qp), x1 = *reinterpret_cast<const float4*>(qp + 4);
@@ -236,20 +237,22 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
   // branch, so a wait counts the loads behind the one it is for)
   Blk blk;
   int key = 0, limit = 0;
+  Base at0;   // where the block's cache lies
   auto next = [&](int b) {
     w.block(b, key, limit);
+    at0 = w.base(b);
     if (b >= w.nb) key = limit = 0;
   };
   next(b0);
-  blk.load_k(w, key, limit, n, kq);
-  blk.template load_v<0, 8>(w, key, limit, n, kq);
+  blk.load_k(at0, key, limit, n, kq);
+  blk.template load_v<0, 8>(at0, key, limit, n, kq);
   __builtin_amdgcn_sched_barrier(0);
 
   // q times the softmax's scale and log2 e, a row's largest magnitude brought to
   // [2^13, 2^14), in two parts
 #pragma unroll
   for (int u = 0; u < kTurns; ++u) {
-    const int i = tid + u * kW * 64, r = i / (HD / 8), c = i % (HD / 8);
+    const int i = tid + u * W * 64, r = i / (HD / 8), c = i % (HD / 8);
     if (i < kChunks) {
       const bool live = rows.r0 + r < rows.r1;
       float amax = 0.f;
@@ -329,7 +332,7 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
       for (int t = 0; t < NT; ++t)
         d[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(blk.k_slice(u, c), low ? ql[PACK ? 0 : t][PACK ? 0 : c] : qh[t][c], d[t][u], 0, 0, 0);
       if constexpr (!FIRST && (i + 1) * 8 / kGroups > i * 8 / kGroups) {
-        blk.template load_v<i * 8 / kGroups, (i + 1) * 8 / kGroups>(w, key, limit, n, kq);
+        blk.template load_v<i * 8 / kGroups, (i + 1) * 8 / kGroups>(at0, key, limit, n, kq);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -344,7 +347,7 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
     const int at = key, end = limit;
     __builtin_amdgcn_sched_barrier(0);
     next(b + step);
-    blk.load_k(w, key, limit, n, kq);
+    blk.load_k(at0, key, limit, n, kq);
     __builtin_amdgcn_sched_barrier(0);
 
     // the softmax of all tiles in straight code but for what happens seldom: a
@@ -498,16 +501,16 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
   __syncthreads();
   constexpr int kQuads = HD / 4;
   static_assert(kRows * kQuads % 64 == 0, "whole waves");
-  for (int i = tid; i < kRows * kQuads; i += kW * 64) {
+  for (int i = tid; i < kRows * kQuads; i += W * 64) {
     const int r = i / kQuads, c = i % kQuads, all = rows.r0 + r;
     const bool live = all < rows.r1;
     float mx = -INFINITY, lt = 0.f;
 #pragma unroll
-    for (int k = 0; k < kW; ++k) mx = fmaxf(mx, sh.r.m[k][r]);
+    for (int k = 0; k < W; ++k) mx = fmaxf(mx, sh.r.m[k][r]);
     const float mo = mx == -INFINITY ? 0.f : mx;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < kW; ++k) {
+    for (int k = 0; k < W; ++k) {
       lt += sh.r.l[k][r] * pow2(sh.r.m[k][r] - mo);
       const float f = pow2(sh.r.e[k][r] - kPExp - mo);
       const float4 v = *reinterpret_cast<const float4*>(&sh.r.o[k][r][4 * c]);
@@ -621,6 +624,36 @@ __global__ void __launch_bounds__(kW * 64, simd_waves(HD)) k_span_shared(const S
   }
 }
 
+// The prefix's blocks, then a sequence's own.
+struct SharedWalk : Walk {
+  Base own;
+  __device__ __forceinline__ Base base(int b) const { return b < nb0 ? Base(*this) : own; }
+};
+// A sequence's rows over both caches in one workgroup. Grid: n_kv_heads x sequences.
+template <int HD, int KVT, bool CAP>
+__global__ void __launch_bounds__(kWide * 64, simd_waves(HD)) k_span_each(const SpanArgs a) {
+  __shared__ Joint<HD, 0, kWide> sh;
+  const int kvh = blockIdx.x % a.n_kv_heads, t = blockIdx.x / a.n_kv_heads;
+  const size_t base = (size_t)kvh * a.max_seq * Block<HD, KVT>::kRowB;
+  const size_t own = ((size_t)t * a.n_kv_heads + kvh) * a.own_max * Block<HD, KVT>::kRowB;
+  SharedWalk w;
+  w.k = static_cast<const uint8_t*>(a.kc) + base;
+  w.v = static_cast<const uint8_t*>(a.vc) + base;
+  w.ks = a.ks;
+  w.vs = a.vs;
+  w.own.k = static_cast<const uint8_t*>(a.ko) + own;
+  w.own.v = static_cast<const uint8_t*>(a.vo) + own;
+  w.own.ks = a.kos + (size_t)t * a.own_max;
+  w.own.vs = a.vos + (size_t)t * a.own_max;
+  w.to0 = a.prefix;
+  w.from1 = 0;
+  w.to1 = own_length(a, t);
+  w.nb0 = blocks_of(w.to0);
+  w.nb = w.nb0 + blocks_of(w.to1);
+  const Rows r = {t << a.gs, t + 1 << a.gs, kvh};
+  span_tile<HD, KVT, 0, CAP, kWide>(a, r, w, 0, 1, nullptr, nullptr, sh, TailMask{});
+}
+
 // The slots' shares -> outputs: a thread takes four outputs of a row from every
 // `groups`-th slot, and the groups of a row meet in LDS.
 constexpr int kJoinThreads = 256;
@@ -681,6 +714,7 @@ int up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // rows' kernel (ss_flash_span.hip).
 struct Plan {
   int rt, tiles, np, no;
+  bool each = false;   // k_span_each
 };
 int rt_of(int hd, int64_t rows) { return rows <= 8 ? 0 : rows <= 16 || hd == 256 ? 1 : 2; }
 // workgroups that a device holds at once
@@ -742,6 +776,13 @@ int most_window_slots(int hd, int group, int n_kv_heads, int n, int64_t first, i
 Plan plan_shared(int hd, int group, int n_kv_heads, int n, int prefix, int own_max, int n_cu) {
   const int64_t rows = (int64_t)n * group, nbp = up(prefix, kKeys), nbo = up(own_max, kKeys);
   Plan p;
+  // Short caches: a workgroup per sequence and KV head goes through both, prefix and
+  // all, and nothing is joined, if that is one workgroup per compute unit at most
+  // (32 heads on 8, head_dim 128, in us, and in tiles: 16 sequences, 11 blocks 6.3
+  // and 10.9; 16 blocks 7.0 and 11.8; 29 blocks 11.4 and 12.1; 4 sequences, 29 blocks
+  // 11.2 and 8.7; 37, 11 blocks 10.0 and 11.5; 16 with K and V per head, int8, 14
+  // blocks 13.1 and 11.0. head_dim 64, 16 on 4, 26 blocks 7.1 and 9.0).
+  if (hd < 256 && (nbp + nbo) * hd <= 2048 && (int64_t)n * n_kv_heads <= n_cu) return {0, 0, 1, 0, true};
   p.rt = prefix ? rt_of(hd, rows) : 0;
   p.tiles = prefix ? up(rows, tile_rows(p.rt)) : 0;
   // all workgroups at once, if that is not cheaper still with fewer slots
@@ -788,8 +829,20 @@ hipError_t launch_rt(const SpanArgs& a, const Plan& p, hipStream_t s) {
 }
 
 template <int HD, int KVT>
+hipError_t launch_each(const SpanArgs& a, hipStream_t s) {
+  const dim3 block(kWide * 64), grid((unsigned)(a.n_kv_heads * a.n));
+  if (a.softcap > 0.f)
+    hipLaunchKernelGGL((k_span_each<HD, KVT, true>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((k_span_each<HD, KVT, false>), grid, block, 0, s, a);
+  return hipGetLastError();
+}
+
+template <int HD, int KVT>
 hipError_t launch_kv(const SpanArgs& a, const Plan& p, hipStream_t s) {
   hipError_t e = hipErrorInvalidValue;
+  if constexpr (HD < 256)
+    if (p.each) return launch_each<HD, KVT>(a, s);
   if (p.rt < 0) {
     e = launch_flash_span(HD, KVT, a, p.np, s);
   } else if (p.rt == 0) {

@@ -74,7 +74,7 @@ def test_workspaces(bad):
     x = C.addressof(ctx)
     needs = [("ss_hip_attention_window", dict(WINDOW, max_seq=5000, pos0=4000, window=3000),
               L.ss_hip_attention_window_workspace(x, 8, 2, 64, 2, 3000, 1)),
-             ("ss_hip_attention_shared", SHARED, L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2, 20, 10)),
+             ("ss_hip_attention_shared", dict(SHARED, prefix_max=5000, prefix=4000), L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2, 4000, 10)),
              ("ss_hip_sample_rows", dict(SAMPLE, n=100000, ld=100000), L.ss_hip_sample_rows_workspace(x, 2, 100000))]
     for name, good, need in needs:
         assert need > 0, name

@@ -16,6 +16,10 @@ SHAPES = [
     (8, 4, 128, 33, 90, [90, 1, 0]), (16, 8, 256, 700, 129, [128, 129, 5]), (8, 1, 256, 64, 33, [33, 32]),
     (32, 8, 128, 5000, 1, [1] * 40), (8, 8, 128, 257, 20, list(range(21)) * 4), (32, 4, 64, 1023, 600, [600, 599, 1]),
     (8, 1, 128, 300, 3000, [3000, 2999, 0, 33]), (16, 2, 128, 2000, 5, [5, 4, 3, 2, 1, 0] * 22),
+    # short caches of which one could grow: tiles and shares; at most 16 blocks (32 at head_dim 64): one workgroup for both
+    (32, 8, 128, 31, 700, [700, 5, 0]), (4, 4, 64, 1, 1100, [1, 1100]), (8, 2, 128, 33, 600, [0, 1, 32]),
+    (4, 4, 64, 33, 1500, [40] * 9), (32, 8, 128, 64, 448, [448, 0, 31, 32, 33]), (32, 4, 64, 900, 96, [96, 95, 0, 1]),
+    (8, 8, 128, 1, 30, [0, 1, 30]), (16, 2, 64, 32, 32, [32] * 100), (8, 8, 128, 65, 60, [60, 1] * 32),
 ]
 
 
@@ -54,10 +58,11 @@ def test_lengths_outside_the_cache(hip, kv):
 
 @pytest.mark.parametrize("where", ["prefix", "own"])
 @pytest.mark.parametrize("bad", [np.inf, np.nan])
-def test_a_value_that_is_not_finite_reaches_those_that_see_it(hip, where, bad):
-    print("shared, V not finite", where, bad, flush=True)
+@pytest.mark.parametrize("own_max", [40, 700])
+def test_a_value_that_is_not_finite_reaches_those_that_see_it(hip, where, bad, own_max):
+    print("shared, V not finite", where, bad, own_max, flush=True)
     lens = [20, 40, 3, 17]
-    q, prefix, own = _case(0, 32, 8, 128, 50, 40, lens)
+    q, prefix, own = _case(0, 32, 8, 128, 50, own_max, lens)
     want = shared_exact(q, prefix, 50, own, lens, 0.0)
     if where == "own":
         own[1][1, :, 39] = bad
@@ -72,10 +77,11 @@ def test_a_value_that_is_not_finite_reaches_those_that_see_it(hip, where, bad):
         assert row_err(got[:, :, keep], want[:, :, keep]).max() <= TOL
 
 
-def test_wide_int8_scales(hip):
-    print("shared, wide scales", flush=True)
+@pytest.mark.parametrize("own_max", [60, 700])
+def test_wide_int8_scales(hip, own_max):
+    print("shared, wide scales", own_max, flush=True)
     lens = [1, 60, 33, 2]
-    q, prefix, own = _case(1, 32, 8, 128, 300, 60, lens)
+    q, prefix, own = _case(1, 32, 8, 128, 300, own_max, lens)
     rng = np.random.default_rng(5)
     prefix[3] *= 10.0 ** rng.uniform(-8, 0, prefix[3].shape).astype(np.float32)
     own[3] *= 10.0 ** rng.uniform(-8, 3, own[3].shape).astype(np.float32)

@@ -31,7 +31,7 @@ class Shared:
         self.host = cache(rng, kv, KVH, prefix, HD), cache(rng, kv, KVH, own_max, HD, (seqs,))
         self.pre, self.own = (_up(hip, c) for c in self.host)
         self.q, self.out, self.lens = (hip.buf(n) for n in (4 * seqs * H * HD, 4 * seqs * H * HD, 4 * seqs))
-        self.ws = hip.buf(hip.L.ss_hip_attention_shared_workspace(hip.ctx, H, KVH, HD, seqs, prefix, own_max))
+        self.ws = hip.buf(max(hip.L.ss_hip_attention_shared_workspace(hip.ctx, H, KVH, HD, seqs, prefix, own_max), 16))
 
     def call(self, stream):
         rc = self.hip.L.ss_hip_attention_shared(
@@ -74,11 +74,11 @@ def streams(hip):
         s.free()
 
 
-@pytest.mark.parametrize("kv", [0, 1])
-def test_shared_replayed_with_other_lengths(hip, streams, kv):
+@pytest.mark.parametrize("kv,prefix", [(0, 700), (1, 700), (0, 3000), (1, 3000)])
+def test_shared_replayed_with_other_lengths(hip, streams, kv, prefix):
     """One capture serves every step: queries and lengths are read when it runs."""
-    print("graph, shared, kv", kv, flush=True)
-    c, st = Shared(hip, kv, 5, 700, 90, 1), streams()
+    print("graph, shared, kv", kv, prefix, flush=True)
+    c, st = Shared(hip, kv, 5, prefix, 90, 1), streams()
     run = st.capture(lambda: c.call(st.ptr))
     for step in range(6):
         want = c.set(10 + step)
@@ -96,7 +96,7 @@ def test_shared_replayed_with_other_lengths(hip, streams, kv):
 def test_two_graphs_at_a_time(hip, streams):
     """Two captures with a workspace each, launched on two streams without waiting between."""
     print("graph, two at a time", flush=True)
-    calls, sts = [Shared(hip, 0, 7, 1500, 300, s) for s in (3, 4)], [streams(), streams()]
+    calls, sts = [Shared(hip, 0, 7, 2500, 300, s) for s in (3, 4)], [streams(), streams()]
     wants = [c.set(20 + i) for i, c in enumerate(calls)]
     runs = [st.capture(lambda c=c, st=st: [c.call(st.ptr) for _ in range(4)]) for c, st in zip(calls, sts)]
     for _ in range(5):
