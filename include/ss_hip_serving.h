@@ -9,8 +9,9 @@
  * after. Calls that may run at the same time (two streams, two captured
  * graphs) need workspaces of their own; calls in one stream can share one.
  * Queries, outputs and caches are 16-byte aligned; an output overlaps no
- * input; a cache holds at most 2^30 positions. The workspace functions return 0
- * for a shape that the call refuses. */
+ * input; a cache holds at most 2^30 positions, a call at most 2^24 tokens times
+ * heads or 2^22 sequences times heads. The workspace functions return 0 for a
+ * shape that the call refuses. */
 #ifndef SS_HIP_SERVING_H
 #define SS_HIP_SERVING_H
 

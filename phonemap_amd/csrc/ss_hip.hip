@@ -635,6 +635,8 @@ int32_t span_setup(ss_hip_ctx_t* c, const char* what, ssk::SpanArgs& a, float* o
 
 // positions of a cache that the walks' 32-bit keys, some blocks past its end, count
 constexpr int32_t kMaxPositions = 1 << 30;
+// sequences times heads: a workgroup each, whose threads 32 bits count
+constexpr int64_t kMaxSeqRows = 1 << 22;
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 
@@ -790,7 +792,7 @@ int32_t ss_hip_attention_window(ss_hip_ctx_t* c, float* out, const float* q, con
 
 size_t ss_hip_attention_shared_workspace(ss_hip_ctx_t* c, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                          int32_t n_seqs, int32_t prefix_len, int32_t own_max) {
-  if (!c || !span_shape_ok(n_heads, n_kv_heads, head_dim, n_seqs) || prefix_len < 0 || prefix_len > kMaxPositions ||
+  if (!c || !span_shape_ok(n_heads, n_kv_heads, head_dim, n_seqs) || (int64_t)n_seqs * n_heads > kMaxSeqRows || prefix_len < 0 || prefix_len > kMaxPositions ||
       own_max <= 0 || own_max > kMaxPositions)
     return 0;
   return ssk::span_shared_workspace(head_dim, n_heads / n_kv_heads, n_kv_heads, n_seqs, prefix_len, own_max, c->n_cu);
@@ -803,7 +805,8 @@ int32_t ss_hip_attention_shared(ss_hip_ctx_t* c, float* out, const float* q, con
                                 int32_t n_kv_heads, int32_t head_dim, float softcap, int32_t kv_type, void* ws,
                                 size_t ws_bytes, void* stream) {
   if (!c || !k_own || !v_own || !own_len || n_seqs <= 0 || own_max <= 0 || prefix_len < 0 || prefix_len > prefix_max ||
-      prefix_max > kMaxPositions || own_max > kMaxPositions || (prefix_len > 0 && (!k_prefix || !v_prefix)))
+      prefix_max > kMaxPositions || own_max > kMaxPositions || (int64_t)n_seqs * n_heads > kMaxSeqRows ||
+      (prefix_len > 0 && (!k_prefix || !v_prefix)))
     return fail(kErrParams, "attention_shared: bad argument (%d sequences, prefix %d of %d, own_max %d)", n_seqs, prefix_len,
                 prefix_max, own_max);
   ssk::SpanArgs a;

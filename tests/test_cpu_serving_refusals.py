@@ -90,6 +90,9 @@ def test_workspaces_of_refused_shapes():
     assert L.ss_hip_attention_window_workspace(x, 8, 2, 64, 2 ** 31 - 1, 3000, 1) == 0
     assert L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2, -1, 10) == 0
     assert L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2 ** 31 - 1, 10, 10) == 0
+    assert L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2 ** 19, 10, 10) > 0
+    assert L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2 ** 19 + 1, 10, 10) == 0
+    assert L.ss_hip_attention_shared_workspace(x, 8, 2, 64, 2, 2 ** 30 + 1, 10) == 0
     assert L.ss_hip_sample_rows_workspace(x, 65536, 100000) == 0
     assert L.ss_hip_sample_rows_workspace(x, 2, 1 << 19) == 0
 
@@ -121,7 +124,8 @@ def test_window_limits(bad):
 
 
 @pytest.mark.parametrize("bad", [dict(prefix_max=2 ** 30 + 1), dict(prefix_max=2 ** 31 - 1, prefix=2 ** 31 - 1),
-                                 dict(own_max=2 ** 30 + 1), dict(own_max=2 ** 31 - 1), dict(cap=1e-40)], ids=str)
+                                 dict(own_max=2 ** 30 + 1), dict(own_max=2 ** 31 - 1), dict(cap=1e-40),
+                                 dict(seqs=2 ** 19 + 1), dict(seqs=2 ** 31 - 1)], ids=str)
 def test_shared_limits(bad):
     _refused("ss_hip_attention_shared", SHARED, **bad)
 
