@@ -19,8 +19,9 @@
 // reach e^-31.75, where all entries together weigh less than 2^-26. The highest
 // of the three thresholds lies in one bin; what lies above that bin stays, what
 // lies below goes, and the bin's own entries are gathered and the threshold found
-// among them. A bin with more than kList of them (equal logits), or |x / T| past
-// 2^18, leaves the row to `slow`, which selects by the bits of x over the whole row.
+// among them. Of a bin with more than kList of them (flat rows) one workgroup goes
+// through the whole row for it. |x / T| past 2^18 leaves the row to `slow`, which
+// selects by the bits of x without bins.
 //
 // Rows of up to kOne entries: one workgroup with the row in registers, one launch.
 // Longer ones: a launch over tiles for their maxima and histograms, and one with
@@ -40,7 +41,9 @@ namespace {
 
 constexpr double kUnit = 17592186044416.0;  // 2^44
 constexpr int kBins = 128;
-constexpr int kCopies = 8;                  // of the histogram, one per lane % 8
+// Of the histogram, one per lane % 4 (64 rows of 128256, top-p: one copy 39.7 us, two
+// 39.8, four 39.9, eight 40.9; of entries in few bins, top-k: 57, 44, 38, 37).
+constexpr int kCopies = 4;
 constexpr int kList = 8192;                 // entries of the threshold's bin
 constexpr int kPairs = 256;                 // up to this many are compared each with all
 constexpr float kFar = 1048576.f;           // 2^20 bins from 0: neighbours are not told apart
@@ -180,19 +183,20 @@ __device__ __forceinline__ void add_u64(uint64_t* p, uint64_t v) {
 }
 
 // Selection by the bits of the keys, kDigit at a time: the largest key at which
-// the sum of val(i) over the entries i < n with that key or a greater one reaches
+// the sum of val(x) over the entries with that key or a greater one reaches
 // target, or a smaller one that parts the entries alike, 0 when all together do
-// not. one: what one entry's val is at most, and less than two entries' (0: not
-// known). hist: 2^kDigit words, red: NT / 64 + 3.
+// not. entries(f): f(x) of each of this thread's entries; some: one of all. one:
+// what one entry's val is at most, and less than two entries' (0: not known).
+// hist: 2^kDigit words, red: NT / 64 + 3.
 constexpr int kDigit = 10, kDigits = 1 << kDigit;
-template <int NT, class Key, class Val>
-__device__ uint32_t key_reaching(int n, uint64_t target, uint64_t one, uint64_t* hist, uint64_t* red, Key key, Val val) {
+template <int NT, class Entries, class Val>
+__device__ uint32_t key_reaching(float some, uint64_t target, uint64_t one, uint64_t* hist, uint64_t* red, Entries entries, Val val) {
   constexpr int kEach = kDigits / NT;   // digits of a thread, the highest ones in thread 0
   static_assert(kEach * NT == kDigits, "whole");
   // the bits that all keys share
-  const uint32_t first = key(0);
+  const uint32_t first = order(some);
   uint32_t differ = 0;
-  for (int i = threadIdx.x; i < n; i += NT) differ |= key(i) ^ first;
+  entries([&](float x) { differ |= order(x) ^ first; });
   for (int d = threadIdx.x; d < kDigits; d += NT) hist[d] = 0;
   int shift = (int)group_max<NT>(differ ? 32 - __clz((int)differ) : 0, red);   // as many low bits do not
   uint64_t* found = red + NT / 64;
@@ -202,10 +206,10 @@ __device__ uint32_t key_reaching(int n, uint64_t target, uint64_t one, uint64_t*
     const int bits = min(kDigit, shift);
     shift -= bits;
     const uint32_t digit = (1u << bits) - 1;
-    for (int i = threadIdx.x; i < n; i += NT) {
-      const uint32_t k = key(i);
-      if ((k & mask) == prefix) add_u64(&hist[(k >> shift) & digit], val(i));
-    }
+    entries([&](float x) {
+      const uint32_t k = order(x);
+      if ((k & mask) == prefix) add_u64(&hist[(k >> shift) & digit], val(x));
+    });
     if (threadIdx.x == 0) found[0] = kDigits;
     __syncthreads();
     uint64_t h[kEach], sum = 0, all;
@@ -359,6 +363,24 @@ struct Chunk {
   }
 };
 
+// f(i, x[i]) of each of this thread's entries of a row, 4 of them requested at a
+// time (64 hot rows of 128256 234 us, one at a time 950; eight 267, but every other
+// row then takes 49 us instead of 40, for the code and registers of it)
+template <int NT, class F>
+__device__ __forceinline__ void over_row(const float* x, int V, F f) {
+  using Round = Chunk<NT, 4>;
+#pragma unroll 1
+  for (int i0 = 0; i0 < V; i0 += 4 * NT) {
+    Round c;
+    c.load(x, i0, V);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + Round::at(e / 4, e % 4);
+      if (i < V) f(i, c.x[e]);
+    }
+  }
+}
+
 // ---- the thresholds --------------------------------------------------------------
 // Where the highest of the thresholds lies, from the bins' entries and weights.
 struct Edge {
@@ -418,7 +440,20 @@ __device__ __forceinline__ Edge find_edge(const SampleRowsArgs& a, const Bins& h
   return {r, kb == r ? need_k : 0, pb == r ? need_p : 0};
 }
 
-// The least key that stays, among the n entries of the threshold's bin (v: their
+// The least key that stays, among the entries of the threshold's bin
+template <int NT, class Entries>
+__device__ uint32_t least_among(const Edge& e, const Keep& keep, float some, uint64_t* digits, uint64_t* red, Entries entries) {
+  const float bin = keep.top - (float)e.r;
+  uint32_t k = 0;
+  // (weights are e^-1/8 .. e^1/8 times 2^44, and a little)
+  constexpr uint64_t kOneWeight = 3ull << 43;
+  if (e.need_k) k = key_reaching<NT>(some, e.need_k, 1, digits, red, entries, [](float) { return 1ull; });
+  if (e.need_p)
+    k = max(k, key_reaching<NT>(some, e.need_p, kOneWeight, digits, red, entries, [&](float x) { return keep.scale.units(x, bin); }));
+  return k;
+}
+
+// The same, of the n entries of that bin (v: their
 // logits, in LDS): each compared with all, by 8 threads, or selection by bits.
 // digits: kDigits words.
 template <int NT>
@@ -457,30 +492,26 @@ __device__ uint32_t least_of(const Edge& e, const Keep& keep, const float* v, in
     __syncthreads();
     return *least;
   }
-  auto key = [&](int i) { return order(v[i]); };
-  uint32_t k = 0;
-  // (weights are e^-1/8 .. e^1/8 times 2^44, and a little)
-  constexpr uint64_t kOneWeight = 3ull << 43;
-  if (e.need_k) k = key_reaching<NT>(n, e.need_k, 1, digits, red, key, [](int) { return 1ull; });
-  if (e.need_p) k = max(k, key_reaching<NT>(n, e.need_p, kOneWeight, digits, red, key, [&](int i) { return keep.scale.units(v[i], bin); }));
-  return k;
+  return least_among<NT>(e, keep, v[0], digits, red, [&](auto f) {
+    for (int i = tid; i < n; i += NT) f(v[i]);
+  });
 }
 
 // A whole row by one workgroup without bins, with weights of up to 2^44.
 template <int NT>
 __device__ int slow(const SampleRowsArgs& a, const float* x, float mx, float u, uint64_t* hist, uint64_t* red) {
   const int V = a.V, tid = threadIdx.x;
-  auto key = [&](int i) { return order(x[i]); };
-  auto weight = [&](int i) { return (uint64_t)(exp(gap(x[i], mx) / a.temperature) * kUnit + 0.5); };
+  auto entries = [&](auto f) { over_row<NT>(x, V, [&](int, float y) { f(y); }); };
+  auto weight = [&](float y) { return (uint64_t)(exp(gap(y, mx) / a.temperature) * kUnit + 0.5); };
   uint32_t least = 0;
-  if (a.top_k) least = key_reaching<NT>(V, (uint64_t)a.top_k, 1, hist, red, key, [](int) { return 1ull; });
+  if (a.top_k) least = key_reaching<NT>(mx, (uint64_t)a.top_k, 1, hist, red, entries, [](float) { return 1ull; });
   if (a.top_p < 1.0) {
     uint64_t s = 0;
-    for (int i = tid; i < V; i += NT) s += weight(i);
+    entries([&](float y) { s += weight(y); });
     const double goal = ceil(a.top_p * (double)group_sum<NT>(s, red));
-    least = max(least, key_reaching<NT>(V, (uint64_t)fmax(goal, 1.0), 0, hist, red, key, weight));
+    least = max(least, key_reaching<NT>(mx, (uint64_t)fmax(goal, 1.0), 0, hist, red, entries, weight));
   }
-  auto kept = [&](int i) { return key(i) >= least && gap(x[i], mx) >= a.min_gap ? weight(i) : 0; };
+  auto kept = [&](int i) { return order(x[i]) >= least && gap(x[i], mx) >= a.min_gap ? weight(x[i]) : 0; };
   // contiguous pieces: the thread in whose piece the running sum passes the draw
   const int C = (V + NT - 1) / NT, i0 = min(tid * C, V), i1 = min(i0 + C, V);
   uint64_t s = 0, total;
@@ -818,15 +849,23 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
       }
       __syncthreads();
     }
-    if (n > kList) {
-      const int i = slow<NT>(a, x, mx, u, digits, red);
-      if (tid == 0) a.out[row] = i;
-      return;
+    if (n > kList) {   // more than the list holds: through the row again
+      auto in_bin = [&](auto f) {
+        over_row<NT>(x, a.V, [&](int i, float y) {
+          if (floorf(y * scale.per) == bin) f(i, y);
+        });
+      };
+      if (e.inside())
+        keep.least = fmaxf(keep.least, from_order(least_among<NT>(e, keep, v[0], digits, red, [&](auto f) { in_bin([&](int, float y) { f(y); }); })));
+      in_bin([&](int i, float y) {
+        if (y >= keep.least) add_u64(&edge_kept[i / kTile], scale.units(y, bin));
+      });
+    } else {
+      if (e.inside())   // (else min-p alone cuts there)
+        keep.least = fmaxf(keep.least, from_order(least_of<NT>(e, keep, v, n, digits, red, &least)));
+      for (int i = tid; i < n; i += NT)
+        if (v[i] >= keep.least) add_u64(&edge_kept[at[i] / kTile], scale.units(v[i], bin));
     }
-    if (e.inside())   // (else min-p alone cuts there)
-      keep.least = fmaxf(keep.least, from_order(least_of<NT>(e, keep, v, n, digits, red, &least)));
-    for (int i = tid; i < n; i += NT)
-      if (v[i] >= keep.least) add_u64(&edge_kept[at[i] / kTile], scale.units(v[i], bin));
     __syncthreads();
     for (int t = tid; t < tiles; t += NT) kept[t] += (double)edge_kept[t] * (1.0 / kUnit) * fall[e.r];
     __syncthreads();

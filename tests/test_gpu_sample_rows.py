@@ -98,3 +98,17 @@ def test_draws_follow_the_weights(hip):
     x = np.repeat(np.log(np.array([[1, 2, 4, 8, 1]], np.float32)), 1600, 0)
     got = sample_call(hip, x, 1.0, 0, 1.0, 0.0, (np.arange(1600) + 0.5) / 1600)
     assert np.all(np.abs(np.bincount(got, minlength=5) - 100 * np.array([1, 2, 4, 8, 1])) <= 1)
+
+
+@pytest.mark.parametrize("setting", [(6.0, 0, 0.9, 0.0), (6.0, 20000, 1.0, 0.0), (4.0, 30000, 0.7, 0.001), (40.0, 1, 1.0, 0.0),
+                                     (40.0, 0, 0.999, 0.0), (9.0, 128000, 0.0, 0.3)], ids=str)
+def test_more_entries_near_the_threshold_than_the_list_holds(hip, setting):
+    """High temperatures bring tens of thousands of different logits within a quarter of one another."""
+    print("sample rows, hot", setting, flush=True)
+    rng = np.random.default_rng(int(10 * setting[0]))
+    x = (2.5 * rng.standard_normal((5, 128256))).astype(np.float32)
+    x[1, ::7] = np.nan
+    x[2, ::2] = np.float32(0.5)
+    u = rng.random(5, np.float32)
+    u[3:] = 0.0, np.float32(1 - 2 ** -24)
+    assert _check(hip, x, setting, u) <= 1
