@@ -792,7 +792,8 @@ int32_t ss_hip_attention_window(ss_hip_ctx_t* c, float* out, const float* q, con
 
 size_t ss_hip_attention_shared_workspace(ss_hip_ctx_t* c, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                          int32_t n_seqs, int32_t prefix_len, int32_t own_max) {
-  if (!c || !span_shape_ok(n_heads, n_kv_heads, head_dim, n_seqs) || (int64_t)n_seqs * n_heads > kMaxSeqRows || prefix_len < 0 || prefix_len > kMaxPositions ||
+  if (!c || !span_shape_ok(n_heads, n_kv_heads, head_dim, n_seqs) || (int64_t)n_seqs * n_heads > kMaxSeqRows ||
+      prefix_len < 0 || prefix_len > kMaxPositions ||
       own_max <= 0 || own_max > kMaxPositions)
     return 0;
   return ssk::span_shared_workspace(head_dim, n_heads / n_kv_heads, n_kv_heads, n_seqs, prefix_len, own_max, c->n_cu);

@@ -190,7 +190,8 @@ __device__ __forceinline__ void add_u64(uint64_t* p, uint64_t v) {
 // hist: 2^kDigit words, red: NT / 64 + 3.
 constexpr int kDigit = 10, kDigits = 1 << kDigit;
 template <int NT, class Entries, class Val>
-__device__ uint32_t key_reaching(float some, uint64_t target, uint64_t one, uint64_t* hist, uint64_t* red, Entries entries, Val val) {
+__device__ uint32_t key_reaching(float some, uint64_t target, uint64_t one, uint64_t* hist, uint64_t* red, Entries entries,
+                                 Val val) {
   constexpr int kEach = kDigits / NT;   // digits of a thread, the highest ones in thread 0
   static_assert(kEach * NT == kDigits, "whole");
   // the bits that all keys share
@@ -449,7 +450,8 @@ __device__ uint32_t least_among(const Edge& e, const Keep& keep, float some, uin
   constexpr uint64_t kOneWeight = 3ull << 43;
   if (e.need_k) k = key_reaching<NT>(some, e.need_k, 1, digits, red, entries, [](float) { return 1ull; });
   if (e.need_p)
-    k = max(k, key_reaching<NT>(some, e.need_p, kOneWeight, digits, red, entries, [&](float x) { return keep.scale.units(x, bin); }));
+    k = max(k, key_reaching<NT>(some, e.need_p, kOneWeight, digits, red, entries,
+                                [&](float x) { return keep.scale.units(x, bin); }));
   return k;
 }
 
@@ -855,8 +857,10 @@ __global__ void __launch_bounds__(kRowThreads) k_draw(const SampleRowsArgs a, in
           if (floorf(y * scale.per) == bin) f(i, y);
         });
       };
-      if (e.inside())
-        keep.least = fmaxf(keep.least, from_order(least_among<NT>(e, keep, v[0], digits, red, [&](auto f) { in_bin([&](int, float y) { f(y); }); })));
+      if (e.inside()) {
+        auto entries = [&](auto f) { in_bin([&](int, float y) { f(y); }); };
+        keep.least = fmaxf(keep.least, from_order(least_among<NT>(e, keep, v[0], digits, red, entries)));
+      }
       in_bin([&](int i, float y) {
         if (y >= keep.least) add_u64(&edge_kept[i / kTile], scale.units(y, bin));
       });

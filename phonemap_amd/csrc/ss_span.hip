@@ -330,7 +330,8 @@ __device__ __forceinline__ void span_tile(const SpanArgs& a, const Rows& rows, c
       constexpr bool low = !PACK && i < NC * 2;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
-        d[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(blk.k_slice(u, c), low ? ql[PACK ? 0 : t][PACK ? 0 : c] : qh[t][c], d[t][u], 0, 0, 0);
+        d[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(blk.k_slice(u, c), low ? ql[PACK ? 0 : t][PACK ? 0 : c] : qh[t][c],
+                                                         d[t][u], 0, 0, 0);
       if constexpr (!FIRST && (i + 1) * 8 / kGroups > i * 8 / kGroups) {
         blk.template load_v<i * 8 / kGroups, (i + 1) * 8 / kGroups>(at0, key, limit, n, kq);
         __builtin_amdgcn_sched_barrier(0);
